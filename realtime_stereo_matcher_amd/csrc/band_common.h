@@ -291,9 +291,9 @@ __device__ __forceinline__ int exp_of(float x) { return __builtin_amdgcn_frexp_e
 #define SMCV_FOLD_FMA 1  // band_sl's fused fold: 1/C and 2^kk folded into the exponent's FMA (0:
 #endif                   // the cells scaled one by one; cfg4 volume-free 5 % slower, r05)
 #ifndef SMCV_FOLD_PK
-#define SMCV_FOLD_PK 1  // FoldFma's (band_sl's) per-cell exponent, sum and weighted sum as packed
-#endif                  // fp32 pairs (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32): cfg4 volume-free
-                        // -9 %, cfg2 -4 %, volume kept flat (profiles/r06/ab/r6w_*, round 6)
+#define SMCV_FOLD_PK 1  // FoldFma's (band_sl's) per-cell exponent, sum and weighted sum in pairs of
+#endif                  // cells, with even and odd partial sums.  The library is built without the
+                        // packed fp32 instructions, so each pair is two scalar operations
 #ifndef SMCV_SCHED_IL
 #define SMCV_SCHED_IL 0  // diagnostic: chunks of IL segments dealt round-robin to the XCD groups
 #endif                   // instead of one contiguous range each (IL a multiple of 8)
