@@ -257,6 +257,82 @@ int sm_v4_volume(const void* featL, const void* featR, void* out, int dtype,
                  const float* w3, const float* b3, const float* w4, const float* b4,
                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- matching-transformer operators: what a layer that matches by attention, in place of a cost
+ * volume, is made of.  Tokens are (B, L, heads, D) with D contiguous; a row of a channels-last
+ * feature map is one sequence.  float32, float16 and bfloat16. */
+
+/* Cross attention to states of another length:
+ *   out[b,i,h] = sum_j p_ij value[b,j,kv],  p_i = softmax over the allowed j of
+ *   scale * query[b,i,h] . key[b,j,kv],  kv = h / (H / KV)
+ * query (B, Lq, H, D), key and value (B, Lk, KV, D), KV a divisor of H, D a multiple of 8 up to 128;
+ * out (B, Lq, H, D) contiguous.  Key j of sequence b is allowed for token i when
+ *   - j < key_lengths[b] (int32; values are taken into 0 .. Lk; NULL: Lk),
+ *   - key_mask[b * Lk + j] != 0 (bytes, contiguous (B, Lk); NULL: all), and
+ *   - 0 <= i - j < max_disparity, the band of a cost volume's candidates (0: no band).
+ * A row without an allowed key gives 0 (and -inf in lse).  What keys and values hold at positions
+ * past the length or masked is not read.  lse: NULL or (B, KV, Lq * H / KV) float32, the natural
+ * logarithm of the softmax's sum, row i * (H / KV) + h % (H / KV): what the backward call needs.
+ * Strides: element strides of (batch, token, head), multiples of 16 bytes (NULL: contiguous);
+ * pointers 16-byte aligned.  The workspace (16-byte aligned; 0 bytes: none is used) holds partial
+ * results when few rows attend to many keys. */
+int64_t sm_cross_attention_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV,
+                                           int64_t D);
+int sm_cross_attention(const void* query, const void* key, const void* value, void* out, float* lse,
+                       int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV,
+                       int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, float scale, int64_t max_disparity,
+                       const int32_t* key_lengths, const uint8_t* key_mask, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+/* Its gradients from the output, lse and the output's gradient (strides as above): dquery (B, Lq, H,
+ * D), dkey and dvalue (B, Lk, KV, D), contiguous; those of keys that nothing may attend to are 0.
+ * The same bits on every run. */
+int64_t sm_cross_attention_backward_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV);
+int sm_cross_attention_backward(const void* query, const void* key, const void* value,
+                                const void* out, const float* lse, const void* dout, void* dquery,
+                                void* dkey, void* dvalue, int dtype, int64_t B, int64_t Lq,
+                                int64_t Lk, int64_t H, int64_t KV, int64_t D,
+                                const int64_t* q_strides, const int64_t* k_strides,
+                                const int64_t* v_strides, const int64_t* dout_strides, float scale,
+                                int64_t max_disparity, const int32_t* key_lengths,
+                                const uint8_t* key_mask, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+
+/* Rotary positions: the first R values (R even) of every head of x (B, L, H, D) are R/2 pairs, and
+ * pair n of token t is turned by positions[b,t] * frequencies[n] radians, formed in 64 bits, and
+ * scaled by `amplitude`; the others are copied.  y: (B, L, H, D) contiguous. */
+enum sm_rotary_flags {
+  SM_ROTARY_INTERLEAVED = 1, /* pair n is values 2n and 2n + 1 (else n and n + R/2) */
+  SM_ROTARY_INVERSE = 2,     /* turn back: the gradient of the turn */
+  SM_ROTARY_POS64 = 4        /* positions are int64 (else int32) */
+};
+int sm_rotary(const void* x, const void* positions, const double* frequencies, void* y, int dtype,
+              int64_t B, int64_t L, int64_t H, int64_t D, int64_t R, const int64_t* x_strides,
+              int64_t position_stride /* between batches; 0: shared */, int flags, float amplitude,
+              void* stream);
+
+/* Root-mean-square norm of `rows` rows of C values (1 to 65536), after the residual's addition:
+ *   summed = x + residual in the residual's type (not written, and x itself, for a NULL residual)
+ *   y = summed / sqrt(mean(summed^2) + eps) * weight, in x's type
+ * residual and weight have x's type or float32.  Row strides are in elements; outputs are dense. */
+int sm_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* summed,
+                int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
+                int64_t x_stride, int64_t residual_stride, float eps, void* stream);
+/* The same with y in 8 bits: q = e4m3(y / scale), scale = max |y| / 448 over the row (group 0;
+ * scales (rows)) or over each 128 values (group 128; scales (rows, ceil(C / 128))); 1 where y is 0. */
+int sm_rms_norm_e4m3(const void* x, const void* residual, const void* weight, void* q, float* scales,
+                     void* summed, int dtype, int residual_dtype, int weight_dtype, int64_t rows,
+                     int64_t C, int64_t x_stride, int64_t residual_stride, int64_t group, float eps,
+                     void* stream);
+/* Gradients of sm_rms_norm from `summed` (x for a NULL residual), y's gradient and, unless NULL,
+ * summed's (in summed's type): dx in x's type (`dtype`); dresidual float32, or NULL where the stream
+ * has x's type (the residual's gradient then is dx); dweight in the weight's type. */
+int64_t sm_rms_norm_backward_workspace_bytes(int64_t rows, int64_t C);
+int sm_rms_norm_backward(const void* summed, const void* weight, const void* dy, const void* dsummed,
+                         void* dx, void* dresidual, void* dweight, int dtype, int summed_dtype,
+                         int weight_dtype, int64_t rows, int64_t C, int64_t summed_stride,
+                         int64_t dy_stride, int64_t dsummed_stride, float eps, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,7 +18,10 @@ SM_FUSED_DISP_F32 = 2
 SM_FUSED_EXACT_ACC = 4
 SM_IP_AUTO, SM_IP_VALU, SM_IP_MFMA_F32, SM_IP_MFMA_H2, SM_IP_MFMA_H2DB, SM_IP_MFMA_RS, SM_IP_MFMA_SL = 0, 1, 2, 5, 8, 11, 12
 
+SM_ROTARY_INTERLEAVED, SM_ROTARY_INVERSE, SM_ROTARY_POS64 = 1, 2, 4
+
 _p = ctypes.c_void_p
+_f = ctypes.c_float
 _i = ctypes.c_int
 _l = ctypes.c_int64
 _lp = ctypes.POINTER(ctypes.c_int64)
@@ -46,10 +49,22 @@ SIGNATURES = {
     "sm_warp_by_flow_ws": [_p, _p, _p, _i, _l, _l, _l, _l, _l, _l, _l, _lp, _lp, _p, _l, _p],
     "sm_v4_volume_workspace_bytes": [_l, _l, _l],
     "sm_v4_volume": [_p, _p, _p, _i, _l, _l, _l, _l, _l, _lp, _lp] + [_p] * 9 + [_l, _p],
+    "sm_cross_attention_workspace_bytes": [_l] * 6,
+    "sm_cross_attention": [_p] * 5 + [_i] + [_l] * 6 + [_lp] * 3 + [_f, _l, _p, _p, _p, _l, _p],
+    "sm_cross_attention_backward_workspace_bytes": [_l] * 4,
+    "sm_cross_attention_backward": [_p] * 9 + [_i] + [_l] * 6 + [_lp] * 4 + [_f, _l, _p, _p, _p, _l, _p],
+    "sm_rotary": [_p] * 4 + [_i] + [_l] * 5 + [_lp, _l, _i, _f, _p],
+    "sm_rms_norm": [_p] * 5 + [_i] * 3 + [_l] * 4 + [_f, _p],
+    "sm_rms_norm_e4m3": [_p] * 6 + [_i] * 3 + [_l] * 5 + [_f, _p],
+    "sm_rms_norm_backward_workspace_bytes": [_l, _l],
+    "sm_rms_norm_backward": [_p] * 7 + [_i] * 3 + [_l] * 5 + [_f, _p, _l, _p],
 }
 _RESTYPE = {"sm_last_error": ctypes.c_char_p, "sm_v4_volume_workspace_bytes": ctypes.c_int64,
             "sm_warp_by_flow_workspace_bytes": ctypes.c_int64,
-            "sm_cv_inner_product_softargmin_workspace_bytes": ctypes.c_int64}
+            "sm_cv_inner_product_softargmin_workspace_bytes": ctypes.c_int64,
+            "sm_cross_attention_workspace_bytes": ctypes.c_int64,
+            "sm_cross_attention_backward_workspace_bytes": ctypes.c_int64,
+            "sm_rms_norm_backward_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -85,6 +100,14 @@ def check(rc, what):
     if rc != SM_OK:
         msg = load().sm_last_error().decode(errors="replace")
         raise StereoCVError(f"{what} failed (status {rc}): {msg}")
+
+
+_int64x3 = ctypes.c_int64 * 3
+
+
+def int64s(a, b, c):
+    """Three values as an int64[3] for the C ABI."""
+    return _int64x3(a, b, c)
 
 
 def strides_arg(t):

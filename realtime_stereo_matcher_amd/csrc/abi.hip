@@ -1,4 +1,5 @@
 // extern "C" entry points of libstereocv.so (declared in include/stereocv.h).
+#include "attn_common.h"
 #include "common.h"
 
 namespace smcv {
@@ -46,6 +47,18 @@ int warp_entry(const void* image, const void* flow, void* out, int dtype, int64_
                const int64_t* image_strides, const int64_t* flow_strides, void* stream,
                void* workspace, int64_t workspace_bytes);
 int64_t warp_workspace_bytes(int64_t N, int64_t C, int64_t Hi, int64_t Wi, int64_t flow_channels);
+int rotary_entry(const void* x, const void* positions, const double* frequencies, void* y, int dtype,
+                 int64_t B, int64_t L, int64_t H, int64_t D, int64_t R, const int64_t* x_strides,
+                 int64_t position_stride, int flags, float amplitude, void* stream);
+int rms_norm_entry(const void* x, const void* residual, const void* weight, void* y, void* summed,
+                   float* scales, int dtype, int res_dtype, int w_dtype, int64_t rows, int64_t C,
+                   int64_t x_stride, int64_t r_stride, int64_t group, bool q8, float eps, void* stream);
+int64_t rms_norm_workspace_bytes(int64_t rows, int64_t C);
+int rms_norm_backward_entry(const void* summed, const void* weight, const void* dy, const void* dsummed,
+                            void* dx, void* dresidual, void* dweight, int dtype, int s_dtype,
+                            int w_dtype, int64_t rows, int64_t C, int64_t s_stride, int64_t dy_stride,
+                            int64_t ds_stride, float eps, void* workspace, int64_t ws_bytes,
+                            void* stream);
 }  // namespace smcv
 
 using namespace smcv;
@@ -345,4 +358,144 @@ extern "C" int sm_v4_volume(const void* featL, const void* featR, void* out, int
   return v4_volume_entry(static_cast<const float*>(featL), static_cast<const float*>(featR),
                          static_cast<float*>(out), N, C, H, W, D, l_strides, r_strides, w1, b1, w2,
                          b2, w3, b3, w4, b4, workspace, (size_t)workspace_bytes, as_stream(stream));
+}
+
+namespace {
+// the sizes, strides and pointers that both directions of the attention share
+int attention_args(attn::Args* a, const char* what, const void* query, const void* key,
+                   const void* value, int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                   int64_t KV, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                   const int64_t* v_strides, float scale, int64_t max_disparity,
+                   const int32_t* key_lengths, const uint8_t* key_mask) {
+  if (const int rc = attn::check_problem(what, dtype, B, Lq, Lk, H, KV, D, scale, max_disparity)) return rc;
+  if (const int rc = attn::read_strides3(q_strides, Lq, H, D, dtype, query, a->qs, "query")) return rc;
+  if (const int rc = attn::read_strides3(k_strides, Lk, KV, D, dtype, key, a->ks, "key")) return rc;
+  if (const int rc = attn::read_strides3(v_strides, Lk, KV, D, dtype, value, a->vs, "value")) return rc;
+  if (B * Lq * H > 0 && !query) return fail(SM_EINVAL, std::string(what) + ": null query pointer");
+  if (B * Lk * KV > 0 && (!key || !value))
+    return fail(SM_EINVAL, std::string(what) + ": null key or value pointer");
+  a->q = query;
+  a->k = key;
+  a->v = value;
+  a->lengths = key_lengths;
+  a->mask = key_mask;
+  a->B = (int)B;
+  a->Lq = (int)Lq;
+  a->Lk = (int)Lk;
+  a->H = (int)H;
+  a->KV = (int)KV;
+  a->G = KV > 0 ? (int)(H / KV) : 1;
+  a->D = (int)D;
+  a->rows = a->Lq * a->G;
+  a->band = (int)max_disparity;
+  a->splits = 1;
+  a->scale = scale;
+  a->c = scale * attn::kLog2e;
+  return SM_OK;
+}
+}  // namespace
+
+extern "C" int64_t sm_cross_attention_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                                                      int64_t KV, int64_t D) {
+  return attn::fwd_workspace_bytes(B, Lq, Lk, H, KV, D);
+}
+
+extern "C" int sm_cross_attention(const void* query, const void* key, const void* value, void* out,
+                                  float* lse, int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                                  int64_t KV, int64_t D, const int64_t* q_strides,
+                                  const int64_t* k_strides, const int64_t* v_strides, float scale,
+                                  int64_t max_disparity, const int32_t* key_lengths,
+                                  const uint8_t* key_mask, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  SM_ENTRY_BEGIN
+  attn::Args a{};
+  if (const int rc = attention_args(&a, "cross_attention", query, key, value, dtype, B, Lq, Lk, H, KV, D,
+                                    q_strides, k_strides, v_strides, scale, max_disparity, key_lengths,
+                                    key_mask)) return rc;
+  if (workspace_bytes < 0) return fail(SM_EINVAL, "cross_attention: negative workspace size");
+  if (B * Lq * H == 0) return SM_OK;
+  if (!out || reinterpret_cast<uintptr_t>(out) % 16 != 0)
+    return fail(SM_EINVAL, "cross_attention: the output must be 16-byte aligned");
+  a.out = out;
+  a.lse = lse;
+  return attn::fwd_entry(a, dtype, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int64_t sm_cross_attention_backward_workspace_bytes(int64_t B, int64_t Lq, int64_t H,
+                                                               int64_t KV) {
+  return attn::bwd_workspace_bytes(B, Lq, H, KV);
+}
+
+extern "C" int sm_cross_attention_backward(
+    const void* query, const void* key, const void* value, const void* out, const float* lse,
+    const void* dout, void* dquery, void* dkey, void* dvalue, int dtype, int64_t B, int64_t Lq,
+    int64_t Lk, int64_t H, int64_t KV, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+    const int64_t* v_strides, const int64_t* dout_strides, float scale, int64_t max_disparity,
+    const int32_t* key_lengths, const uint8_t* key_mask, void* workspace, int64_t workspace_bytes,
+    void* stream) {
+  SM_ENTRY_BEGIN
+  attn::Args a{};
+  if (const int rc = attention_args(&a, "cross_attention_backward", query, key, value, dtype, B, Lq, Lk,
+                                    H, KV, D, q_strides, k_strides, v_strides, scale, max_disparity,
+                                    key_lengths, key_mask)) return rc;
+  if (const int rc = attn::read_strides3(dout_strides, Lq, H, D, dtype, dout, a.gs, "dout")) return rc;
+  if (workspace_bytes < 0) return fail(SM_EINVAL, "cross_attention_backward: negative workspace size");
+  const bool rows = B * Lq * H > 0, keys = B * Lk * KV > 0;
+  if ((rows && (!out || !lse || !dout || !dquery)) || (keys && (!dkey || !dvalue)))
+    return fail(SM_EINVAL, "cross_attention_backward: null pointer");
+  for (const void* p : {out, static_cast<const void*>(dquery), static_cast<const void*>(dkey),
+                        static_cast<const void*>(dvalue)})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+      return fail(SM_EINVAL, "cross_attention_backward: outputs and gradients must be 16-byte aligned");
+  a.o = out;
+  a.lse = const_cast<float*>(lse);
+  a.dout = dout;
+  a.dq = dquery;
+  a.dk = dkey;
+  a.dv = dvalue;
+  if (!rows && !keys) return SM_OK;
+  return attn::bwd_entry(a, dtype, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int sm_rotary(const void* x, const void* positions, const double* frequencies, void* y,
+                         int dtype, int64_t B, int64_t L, int64_t H, int64_t D, int64_t R,
+                         const int64_t* x_strides, int64_t position_stride, int flags,
+                         float amplitude, void* stream) {
+  SM_ENTRY_BEGIN
+  return rotary_entry(x, positions, frequencies, y, dtype, B, L, H, D, R, x_strides, position_stride,
+                      flags, amplitude, stream);
+}
+
+extern "C" int sm_rms_norm(const void* x, const void* residual, const void* weight, void* y,
+                           void* summed, int dtype, int residual_dtype, int weight_dtype,
+                           int64_t rows, int64_t C, int64_t x_stride, int64_t residual_stride,
+                           float eps, void* stream) {
+  SM_ENTRY_BEGIN
+  return rms_norm_entry(x, residual, weight, y, summed, nullptr, dtype, residual_dtype, weight_dtype,
+                        rows, C, x_stride, residual_stride, 0, false, eps, stream);
+}
+
+extern "C" int sm_rms_norm_e4m3(const void* x, const void* residual, const void* weight, void* q,
+                                float* scales, void* summed, int dtype, int residual_dtype,
+                                int weight_dtype, int64_t rows, int64_t C, int64_t x_stride,
+                                int64_t residual_stride, int64_t group, float eps, void* stream) {
+  SM_ENTRY_BEGIN
+  return rms_norm_entry(x, residual, weight, q, summed, scales, dtype, residual_dtype, weight_dtype,
+                        rows, C, x_stride, residual_stride, group, true, eps, stream);
+}
+
+extern "C" int64_t sm_rms_norm_backward_workspace_bytes(int64_t rows, int64_t C) {
+  return rms_norm_workspace_bytes(rows, C);
+}
+
+extern "C" int sm_rms_norm_backward(const void* summed, const void* weight, const void* dy,
+                                    const void* dsummed, void* dx, void* dresidual, void* dweight,
+                                    int dtype, int summed_dtype, int weight_dtype, int64_t rows,
+                                    int64_t C, int64_t summed_stride, int64_t dy_stride,
+                                    int64_t dsummed_stride, float eps, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  SM_ENTRY_BEGIN
+  return rms_norm_backward_entry(summed, weight, dy, dsummed, dx, dresidual, dweight, dtype,
+                                 summed_dtype, weight_dtype, rows, C, summed_stride, dy_stride,
+                                 dsummed_stride, eps, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,392 @@
+// Cross attention, backward.  With p the weights (formed again from the saved logarithm of their
+// sum), g the output's gradient and delta_i = sum_d g_id o_id:
+//   dv_j = sum_i p_ij g_i      ds_ij = p_ij (g_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
+// Two kernels, each with one side stationary in registers and the other streamed through LDS, so
+// that every sum has one owner: no atomics, the same bits on every run, and the gradients of key
+// heads shared by several query heads are summed in the owner's registers.  That forms the scores
+// and their gradient twice (7 products where one kernel with atomic sums would have 5).
+//   attn_dq   a wave owns 32 query rows; writes dq, and per row delta and the logarithm in base 2
+//   attn_dkv  a wave owns 32 keys; loops over the rows of all heads that share them
+// fp16: ds would fall out of the type's range for small gradients, so g enters with a power of
+// two: one that brings the row's largest |g| into [1/2, 1) in attn_dq (a lane's scalar), the
+// largest of the whole key head in attn_dkv; p enters dv times 2^14.  The factors are exact and are
+// taken out of the fp32 sums at the end.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.h"
+
+namespace smcv {
+namespace attn {
+namespace {
+
+template <typename T, int DP> struct BCfg {
+  static constexpr int kTile = sizeof(T) == 4 || DP == 128 ? 32 : 64;  // streamed rows
+  static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
+  static constexpr int kLdsQ = 4 * kTileBytes;               // two buffers of keys and values
+  static constexpr int kBuf = 2 * kTileBytes + 512;           // rows, gradients, lse and delta
+  static constexpr int kLdsKv = 2 * kBuf;
+};
+
+// the power of two that brings x into [1/2, 1), as an exponent; 0 for 0, infinities and NaN
+__device__ __forceinline__ int down(float x) {
+  const int e = (int)((__float_as_uint(x) >> 23) & 255);
+  return e == 0 || e == 255 ? 0 : min(126 - e, 100);
+}
+
+template <typename T, int DP, bool KMASK>
+__global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dq(Args a) {
+  using C = BCfg<T, DP>;
+  using TL = Tile<T, DP>;
+  using frag = Frag<T>;
+  constexpr int KT = C::kTile, KB = KT / 32;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  unsigned id = xcd_id();
+  const int rt = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int kv = id % a.KV, b = id / a.KV;
+  const int wg_row0 = rt * kRows, row0 = wg_row0 + 32 * wave, row = row0 + (lane & 31);
+  const int token = row / a.G, head = kv * a.G + row % a.G;
+  const bool there = row < a.rows;
+
+  const int keys = key_count(a, b);
+  int jlo = 0, jhi = keys;
+  if (a.band > 0) {
+    const int last = min(wg_row0 + kRows, a.rows) - 1;
+    jlo = max(0, wg_row0 / a.G - a.band + 1);
+    jhi = min(keys, last / a.G + 1);
+  }
+  const int tb = jlo / KT, te = jhi > jlo ? (jhi + KT - 1) / KT : tb;
+
+  const T* K = static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2];
+  const T* V = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
+  const int64_t orow = (((int64_t)b * a.Lq + token) * a.H + head) * a.D;
+  frag q[TL::kSteps], g[TL::kSteps];
+  load_rows<T, DP>(q, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)token * a.qs[1] +
+                          head * a.qs[2], there, half, a.D);
+  load_rows<T, DP>(g, static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)token * a.gs[1] +
+                          head * a.gs[2], there, half, a.D);
+  float delta = 0.f, most = 0.f;
+  {
+    frag o[TL::kSteps];
+    load_rows<T, DP>(o, static_cast<const T*>(a.o) + orow, there, half, a.D);
+#pragma unroll
+    for (int s = 0; s < TL::kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < TL::kPer; ++e) {
+        const float x = Mma<T>::get(g[s], e);
+        delta = fmaf(x, Mma<T>::get(o[s], e), delta);
+        most = fmaxf(most, fabsf(x));
+      }
+    delta = other_half_sum(delta);
+    most = other_half_max(most);
+  }
+  const int64_t n_pad = (int64_t)a.row_tiles * kRows;
+  const int64_t at = ((int64_t)b * a.KV + kv) * n_pad + row;
+  const float lse = there ? a.lse[((int64_t)b * a.KV + kv) * a.rows + row] : -INFINITY;
+  // a row without keys, or past the end: +inf makes every weight that is formed from it 0
+  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
+  if (half == 0) {
+    a.row_lse[at] = lse2;
+    a.row_delta[at] = delta;
+  }
+  int shift = 0;
+  if constexpr (kScaled) {
+    float top = most;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+    if (lane == 0) lds_put(lds_addr(smem) + 4 * wave, top);
+    __syncthreads();
+    if (tid == 0) {
+      const unsigned at0 = lds_addr(smem);
+      a.tile_max[((int64_t)b * a.KV + kv) * a.row_tiles + rt] =
+          fmaxf(fmaxf(lds_get<float>(at0), lds_get<float>(at0 + 4)),
+                fmaxf(lds_get<float>(at0 + 8), lds_get<float>(at0 + 12)));
+    }
+    __syncthreads();
+    shift = down(most);
+    delta = __builtin_ldexpf(delta, shift);
+#pragma unroll
+    for (int s = 0; s < TL::kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < TL::kPer; ++e)
+        Mma<T>::put(g[s], e, __builtin_ldexpf(Mma<T>::get(g[s], e), shift));
+  }
+
+  const unsigned lds = lds_addr(smem);
+  const uint8_t* mask = KMASK ? a.mask + (int64_t)b * a.Lk : nullptr;
+  auto mask_byte = [&](int t) -> int {
+    const int j = t * KT + lane;
+    return lane < KT && t < te && j < keys ? mask[j] : 0;
+  };
+  auto length_bits = [&](int t) -> uint64_t {
+    const int n = keys - t * KT;
+    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+  };
+  constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
+  auto copy = [&](int t, unsigned dst, uint64_t bits) {
+    auto ok = [&](int, int r) { return ((bits >> r) & 1) != 0; };
+    TL::template load<KT, 256>(K, a.ks[1], t * KT, dst, tid, a.D, ok);
+    TL::template load<KT, 256>(V, a.vs[1], t * KT, dst + C::kTileBytes, tid, a.D, ok);
+  };
+
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[db][r] = 0.f;
+
+  uint64_t bits = 0;
+  int byte = 0;
+  if (tb < te) {
+    bits = KMASK ? __ballot(mask_byte(tb)) : length_bits(tb);
+    if (KMASK) byte = mask_byte(tb + 1);
+    copy(tb, lds, bits);
+  }
+  for (int t = tb, buf = 0; t < te; ++t, buf ^= 1) {
+    publish();
+    uint64_t next = 0;
+    if (t + 1 < te) {
+      next = KMASK ? __ballot(byte) : length_bits(t + 1);
+      if (KMASK) byte = mask_byte(t + 2);
+      copy(t + 1, lds + (buf ^ 1) * 2 * C::kTileBytes, next);
+    }
+    const unsigned kt = lds + buf * 2 * C::kTileBytes, vt = kt + C::kTileBytes;
+    const uint64_t seen = bits & kAll;
+    bits = next;
+    bool edge = false;
+    if (a.band > 0) {
+      const int j0 = t * KT, j1 = j0 + KT - 1;
+      const int i0 = row0 / a.G, i1 = min(row0 + 31, a.rows - 1) / a.G;
+      if (j0 > i1 || j1 <= i0 - a.band) continue;
+      edge = j1 > i0 || j0 <= i1 - a.band;
+    }
+    if (seen == 0) continue;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 s = mma_rows<T, DP>(kt, 32 * kb, q, lane);
+      f32x16 ds = mma_rows<T, DP>(vt, 32 * kb, g, lane);
+      if (seen != kAll) {
+        const unsigned w = (unsigned)(seen >> (32 * kb)) >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+      }
+      if (edge) {
+        const int d = token - (t * KT + 32 * kb + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = (unsigned)(d - (8 * (r >> 2) + (r & 3))) < (unsigned)a.band ? s[r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * (ds[r] - delta);
+      mma_transposed<T, DP>(dq, kt, 32 * kb, ds, lane);
+    }
+  }
+  if (!there) return;
+  store_columns<T, DP>(static_cast<T*>(a.dq) + orow, dq, __builtin_ldexpf(a.scale, -shift), half, a.D);
+}
+
+template <typename T, int DP, bool KMASK>
+__global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dkv(Args a) {
+  using C = BCfg<T, DP>;
+  using TL = Tile<T, DP>;
+  using frag = Frag<T>;
+  constexpr int RT = C::kTile, RB = RT / 32;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  constexpr float kUp = kScaled ? 14.f : 0.f;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  unsigned id = xcd_id();
+  const int key_tiles = (a.Lk + kRows - 1) / kRows;
+  const int jt = id % key_tiles;
+  id /= key_tiles;
+  const int kv = id % a.KV, b = id / a.KV;
+  const int wg_j0 = jt * kRows, j0 = wg_j0 + 32 * wave, j = j0 + (lane & 31);
+  const int keys = key_count(a, b);
+  const bool there = j < keys && (!KMASK || a.mask[(int64_t)b * a.Lk + min(j, a.Lk - 1)] != 0);
+
+  frag k[TL::kSteps], v[TL::kSteps];
+  load_rows<T, DP>(k, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)j * a.ks[1] +
+                          kv * a.ks[2], there, half, a.D);
+  load_rows<T, DP>(v, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)j * a.vs[1] +
+                          kv * a.vs[2], there, half, a.D);
+
+  // rows of the heads that share these keys: all, or those whose band reaches them
+  int64_t rlo = 0, rhi = a.rows;
+  if (a.band > 0) {
+    rlo = min((int64_t)a.rows, (int64_t)wg_j0 * a.G);
+    rhi = min((int64_t)a.rows, ((int64_t)min(wg_j0 + kRows, a.Lk) - 1 + a.band) * a.G);
+  }
+  if (wg_j0 >= keys) rhi = rlo;  // nothing attends to them: their gradients are 0
+  const int tb = (int)(rlo / RT), te = rhi > rlo ? (int)((rhi + RT - 1) / RT) : tb;
+
+  const int64_t n_pad = (int64_t)a.row_tiles * kRows;
+  const float* lse = a.row_lse + ((int64_t)b * a.KV + kv) * n_pad;
+  const float* delta = a.row_delta + ((int64_t)b * a.KV + kv) * n_pad;
+  int shift = 0;
+  if constexpr (kScaled) {
+    const float* tm = a.tile_max + ((int64_t)b * a.KV + kv) * a.row_tiles;
+    float top = 0.f;
+    for (int i = lane; i < a.row_tiles; i += 64) top = fmaxf(top, tm[i]);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+    shift = __builtin_amdgcn_readfirstlane(down(top));
+  }
+
+  const unsigned lds = lds_addr(smem);
+  const T* Q = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)kv * a.G * a.qs[2];
+  const T* GO = static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)kv * a.G * a.gs[2];
+  auto copy = [&](int t, unsigned dst) {
+    constexpr int total = RT * TL::kPieces;
+#pragma unroll
+    for (int it = 0; it < (total + 255) / 256; ++it) {
+      if (total % 256 != 0 && it * 256 + wave * 64 >= total) break;
+      const int p = it * 256 + tid, r = p / TL::kPieces;
+      const int ch = (p % TL::kPieces) ^ TL::twist(r);
+      const int row = t * RT + r, token = row / a.G, g = row - token * a.G;
+      const bool ok = row < a.rows && ch * TL::kPer < a.D;
+      const T* qp = Q + (int64_t)token * a.qs[1] + g * a.qs[2] + ch * TL::kPer;
+      const T* gp = GO + (int64_t)token * a.gs[1] + g * a.gs[2] + ch * TL::kPer;
+      copy16(ok ? (const void*)qp : (const void*)g_zero, dst + (it * 256 + wave * 64) * 16);
+      copy16(ok ? (const void*)gp : (const void*)g_zero,
+             dst + C::kTileBytes + (it * 256 + wave * 64) * 16);
+    }
+    // RT logarithms, then RT deltas (the rows are padded to whole tiles there)
+    if (wave == 0) {
+      const float* src = RT == 64 ? lse + t * RT + lane
+                                  : (half ? delta : lse) + t * RT + (lane & 31);
+      copy4(src, dst + 2 * C::kTileBytes);
+    }
+    if (RT == 64 && wave == 1) copy4(delta + t * RT + lane, dst + 2 * C::kTileBytes + 256);
+  };
+
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+
+  if (tb < te) copy(tb, lds);
+  for (int t = tb, buf = 0; t < te; ++t, buf ^= 1) {
+    publish();
+    const unsigned qt = lds + buf * C::kBuf, gt = qt + C::kTileBytes, st = gt + C::kTileBytes;
+    if (t + 1 < te) copy(t + 1, lds + (buf ^ 1) * C::kBuf);
+    if (j0 >= keys) continue;
+    bool edge = false;
+    if (a.band > 0) {
+      const int64_t r0 = (int64_t)t * RT, r1 = r0 + RT - 1;
+      const int64_t first = (int64_t)j0 * a.G, last = ((int64_t)j0 + 31 + a.band) * a.G - 1;
+      if (r1 < first || r0 > last) continue;
+      edge = r0 < (int64_t)(j0 + 31) * a.G || r1 >= ((int64_t)j0 + a.band) * a.G;
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x16 p = mma_rows<T, DP>(qt, 32 * rb, k, lane);
+      f32x16 ds = mma_rows<T, DP>(gt, 32 * rb, v, lane);
+      if (edge) {
+        const int64_t first = (int64_t)j * a.G, width = (int64_t)a.band * a.G;
+        const int64_t off = (int64_t)t * RT + 32 * rb + 4 * half - first;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t x = off + 8 * (r >> 2) + (r & 3);
+          p[r] = x >= 0 && x < width ? p[r] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l4 = lds_get<f32x4>(st + (32 * rb + 8 * g + 4 * half) * 4);
+        const f32x4 d4 = lds_get<f32x4>(st + RT * 4 + (32 * rb + 8 * g + 4 * half) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          // a masked score of -inf against +inf (a row without keys) is still -inf
+          const float w = __builtin_amdgcn_exp2f(fmaf(p[r], a.c, -l4[e]));
+          float x = w * (ds[r] - d4[e]);
+          if constexpr (kScaled) {
+            x = __builtin_ldexpf(x, shift);
+            p[r] = __builtin_ldexpf(w, (int)kUp);
+          } else {
+            p[r] = w;
+          }
+          ds[r] = x;
+        }
+      }
+      mma_transposed<T, DP>(dv, gt, 32 * rb, p, lane);
+      mma_transposed<T, DP>(dk, qt, 32 * rb, ds, lane);
+    }
+  }
+  if (j >= a.Lk) return;
+  const int64_t out = (((int64_t)b * a.Lk + j) * a.KV + kv) * a.D;
+  if (!there) {  // 0 whatever the zero rows that stood for the key gave
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+  }
+  store_columns<T, DP>(static_cast<T*>(a.dv) + out, dv, kScaled ? 0x1p-14f : 1.f, half, a.D);
+  store_columns<T, DP>(static_cast<T*>(a.dk) + out, dk, __builtin_ldexpf(a.scale, -shift), half, a.D);
+}
+
+template <typename T, int DP, bool KMASK>
+int launch(const Args& a, hipStream_t st) {
+  using C = BCfg<T, DP>;
+  static std::atomic<unsigned long long> done_q{0}, done_kv{0};
+  const int dev = stream_device(st);
+  if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK>), C::kLdsQ, dev, done_q)) return rc;
+  if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dkv<T, DP, KMASK>), C::kLdsKv, dev, done_kv)) return rc;
+  const int64_t bkv = (int64_t)a.B * a.KV, key_tiles = ceil_div(a.Lk, kRows);
+  if (bkv * a.row_tiles > 0x7fffffffll || bkv * key_tiles > 0x7fffffffll)
+    return fail(SM_EINVAL, "cross_attention_backward: too many row tiles");
+  if (a.row_tiles > 0) {
+    attn_dq<T, DP, KMASK><<<dim3((unsigned)(bkv * a.row_tiles)), 256, C::kLdsQ, st>>>(a);
+    if (const int rc = check_launch("cross_attention_backward dq")) return rc;
+  }
+  if (key_tiles > 0) {
+    attn_dkv<T, DP, KMASK><<<dim3((unsigned)(bkv * key_tiles)), 256, C::kLdsKv, st>>>(a);
+    return check_launch("cross_attention_backward dk, dv");
+  }
+  return SM_OK;
+}
+
+template <typename T>
+int by_width(const Args& a, hipStream_t st) {
+  const bool km = a.mask != nullptr;
+  if (a.D <= 32) return km ? launch<T, 32, true>(a, st) : launch<T, 32, false>(a, st);
+  if (a.D <= 64) return km ? launch<T, 64, true>(a, st) : launch<T, 64, false>(a, st);
+  return km ? launch<T, 128, true>(a, st) : launch<T, 128, false>(a, st);
+}
+
+}  // namespace
+
+int64_t bwd_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV) {
+  if (B <= 0 || Lq <= 0 || H <= 0 || KV <= 0 || H % KV != 0) return 0;
+  const int64_t tiles = ceil_div(Lq * (H / KV), kRows);
+  return B * KV * tiles * (2 * kRows + 1) * 4;
+}
+
+int bwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st) {
+  a.row_tiles = (int)ceil_div(a.rows, kRows);
+  const int64_t n = (int64_t)a.B * a.KV * a.row_tiles;
+  if (n > 0 && (workspace == nullptr || ws_bytes < n * (2 * kRows + 1) * 4))
+    return fail(SM_EINVAL, "cross_attention_backward: the workspace is smaller than "
+                           "sm_cross_attention_backward_workspace_bytes()");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(SM_EINVAL, "cross_attention_backward: the workspace must be 16-byte aligned");
+  a.row_lse = static_cast<float*>(workspace);
+  a.row_delta = a.row_lse + n * kRows;
+  a.tile_max = a.row_delta + n * kRows;
+  SM_DISPATCH_DTYPE(dtype, T, return by_width<T>(a, st));
+  return SM_OK;
+}
+
+}  // namespace attn
+}  // namespace smcv

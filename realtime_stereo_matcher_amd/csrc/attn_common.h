@@ -1,0 +1,302 @@
+// Shared pieces of the cross-attention kernels (attn_fwd.hip, attn_bwd.hip): the problem, the
+// tiles in LDS and the matrix-instruction operands that are read from them.
+//
+// All products are formed transposed, so that a lane owns one COLUMN of every result.  With the
+// 32x32 result layout (lane l, register r: row 8 (r/4) + 4 (l/32) + r%4, column l%32) a score block
+// S^T = K Q^T leaves each lane 16 keys of one query: the softmax statistics are one scalar a lane,
+// and the same registers, rounded, ARE the right operand of O^T += V^T P^T.  The contraction index
+// of a product may be permuted if both operands agree, so the left operand is read with the order
+// of keys that the result layout happens to have and no value crosses lanes.
+#pragma once
+
+#include "common.h"
+
+namespace smcv {
+namespace attn {
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kCus = 256;    // compute units of the MI355X: what a launch has to fill
+constexpr int kRows = 128;   // query rows of a workgroup (32 a wave)
+constexpr int kFew = 32;     // at most so many rows: the waves share the rows and split the keys
+
+struct Args {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float* lse;             // (B, KV, Lq * G), natural logarithm
+  float *part_o, *part_l; // split keys: (splits, B, KV, rows, D) and (splits, B, KV, rows)
+  float *row_lse, *row_delta;  // backward: (B, KV, padded rows)
+  float* tile_max;        // backward, fp16: largest |dout| of each row tile, (B, KV, row tiles)
+  const int* lengths;     // (B) or null
+  const uint8_t* mask;    // (B, Lk) or null
+  int64_t qs[3], ks[3], vs[3], gs[3];  // element strides of batch, token and head
+  int B, Lq, Lk, H, KV, G, D;
+  int rows, row_tiles;    // Lq * G and its tiles: row r is token r / G, head kv * G + r % G
+  int band;               // > 0: key j is a candidate of token i iff 0 <= i - j < band
+  int splits;
+  float scale, c;         // c = scale * log2(e): exp(scale x) = exp2(c x)
+};
+
+// ------------------------------------------------------------------------------------- operands
+// 16-bit: a 32x32x16 step contracts 16 values, lane l holding 8 of column / row l%32.
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+  using frag = h16x8;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void put(frag& f, int e, float v) { f[e] = (_Float16)v; }
+  static __device__ __forceinline__ float get(const frag& f, int e) { return (float)f[e]; }
+};
+template <> struct Mma<bf16_t> {
+  using frag = b16x8;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void put(frag& f, int e, float v) { f[e] = (__bf16)v; }
+  static __device__ __forceinline__ float get(const frag& f, int e) { return (float)f[e]; }
+};
+// fp32: four 32x32x2 steps a 16-byte piece; step e contracts values 8c + e and 8c + 4 + e.
+template <> struct Mma<float> {
+  using frag = f32x4;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ float get(const frag& f, int e) { return f[e]; }
+};
+
+template <typename T> using Frag = typename Mma<T>::frag;
+
+// ---------------------------------------------------------------------------------- tiles in LDS
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+  return (unsigned)(uintptr_t)(const lds_u8*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_get(unsigned addr) {
+  return *reinterpret_cast<__attribute__((address_space(3))) V*>(addr);
+}
+template <typename V>
+__device__ __forceinline__ void lds_put(unsigned addr, V v) {
+  *reinterpret_cast<__attribute__((address_space(3))) V*>(addr) = v;
+}
+// 16 (4) bytes a lane from global memory into LDS at a wave's base + 16 (4) * lane, without a
+// register in between.  Inline, because the compiler would wait for every such copy in flight
+// before each LDS read; the kernels wait themselves (wait_copies) before the barrier that
+// publishes a tile.
+__device__ __forceinline__ void copy16(const void* src, unsigned dst) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(src), "s"(dst)
+      : "memory");
+}
+__device__ __forceinline__ void copy4(const void* src, unsigned dst) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(src), "s"(dst)
+      : "memory");
+}
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ void publish() {  // this wave's copies done, then everyone's
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// what rows past the end, masked keys and columns past the head's width read instead
+static __device__ const unsigned g_zero[4] = {0, 0, 0, 0};
+
+// A tile of rows x DP values, in 16-byte pieces.  Piece `ch` of row `row` sits at ch ^ twist(row):
+// the 8 rows that a 16-byte read serves at once, and the 4 rows x 32 bytes of a transposing read,
+// then fall on different banks (rows are 64 to 512 bytes apart, a multiple of the bank count).
+template <typename T, int DP> struct Tile {
+  static constexpr int kPer = 16 / (int)sizeof(T);
+  static constexpr int kPieces = DP / kPer;  // of a row
+  static constexpr int kRowBytes = DP * (int)sizeof(T);
+  static constexpr int kSteps = sizeof(T) == 4 ? DP / 8 : DP / 16;  // row-operand reads
+  static __device__ __forceinline__ int twist(int row) {
+    if constexpr (sizeof(T) == 4) return row & 7;
+    if constexpr (kPieces >= 8) return ((row & 3) << 1) | ((row >> 2) & 1);
+    return (row & 2) | ((row >> 2) & 1);
+  }
+  // ROWS rows from `base` (row stride `stride`), row `row0` first, by NT threads (`tid`); `ok(row)`
+  // says which rows of the tile exist.  A wave without a whole instruction left does nothing.
+  template <int ROWS, int NT, typename OK>
+  static __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, unsigned dst,
+                                              int tid, int D, OK ok) {
+    constexpr int total = ROWS * kPieces;
+    static_assert(total % 64 == 0, "whole wave instructions");
+    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+    for (int it = 0; it < (total + NT - 1) / NT; ++it) {
+      if (total % NT != 0 && it * NT + wave0 >= total) break;
+      const int p = it * NT + tid;
+      const int row = p / kPieces;
+      const int ch = (p % kPieces) ^ twist(row);
+      const T* src = base + (int64_t)(row0 + row) * stride + ch * kPer;
+      const bool there = ok(it, row) && ch * kPer < D;
+      copy16(there ? (const void*)src : (const void*)g_zero, dst + (it * NT + wave0) * 16);
+    }
+  }
+  // left operand with the tile's rows as its rows: row `row`, step s
+  static __device__ __forceinline__ Frag<T> row_op(unsigned tile, int row, int s,
+                                                                 int half) {
+    const int ch = (2 * s + half) ^ twist(row);
+    return lds_get<Frag<T>>(tile + row * kRowBytes + ch * 16);
+  }
+};
+
+// registers of a block that hold 4 (fp32) or 8 (16-bit) consecutive contraction steps
+__device__ __forceinline__ int crow(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// acc[db] += (tile rows row0 .. row0+31, transposed) * block, where `block` holds a 32x32 result
+// (tile rows x lane columns): values of the tile's column are the rows of the product.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned tile, int row0,
+                                               const f32x16& block, int lane) {
+  using TL = Tile<T, DP>;
+  if constexpr (sizeof(T) == 4) {
+    const int half = lane >> 5, col = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = row0 + crow(r, half);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        const int ch = (8 * db + (col >> 2)) ^ TL::twist(row);
+        const float a = lds_get<float>(tile + row * TL::kRowBytes + ch * 16 + (col & 3) * 4);
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, block[r], acc[db], 0, 0, 0);
+      }
+    }
+  } else {
+    // ds_read_tr16_b64: in each 16 lanes, lane i receives column i of the 4 x 16 values whose
+    // row j the lanes 4j .. 4j+3 address
+    const int half = lane >> 5, g = (lane >> 4) & 1, l16 = lane & 15;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Frag<T> p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) Mma<T>::put(p, e, block[8 * s + e]);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        s16x4 lo, hi;
+        const int row = 4 * half + (l16 >> 2);
+        const int ch = (4 * db + 2 * g + ((l16 & 3) >> 1)) ^ TL::twist(row);
+        const unsigned at = tile + (row0 + 16 * s + row) * TL::kRowBytes + ch * 16 + (l16 & 1) * 8;
+        typedef __attribute__((address_space(3))) s16x4 lds_s4;
+        lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(at));
+        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_s4*>(at + 8 * TL::kRowBytes));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[db] = Mma<T>::mma(__builtin_bit_cast(Frag<T>, both), p, acc[db]);
+      }
+    }
+  }
+}
+
+// a row in registers, as the right operand of all steps over its values
+template <typename T, int DP> using RowOps = Frag<T>[Tile<T, DP>::kSteps];
+
+// right operand of one row (a query or a key) a lane, straight from global memory
+template <typename T, int DP>
+__device__ __forceinline__ void load_rows(RowOps<T, DP>& f, const T* row, bool there,
+                                          int half, int D) {
+  using TL = Tile<T, DP>;
+#pragma unroll
+  for (int s = 0; s < TL::kSteps; ++s) {
+    const int d = (2 * s + half) * TL::kPer;
+    u32x4 v = {0, 0, 0, 0};
+    if (there && d < D) v = *reinterpret_cast<const u32x4*>(row + d);
+    f[s] = __builtin_bit_cast(Frag<T>, v);
+  }
+}
+
+// the tile's rows row0 .. row0+31 times the lanes' columns
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 mma_rows(unsigned tile, int row0,
+                                           const RowOps<T, DP>& f, int lane) {
+  f32x16 s;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+  for (int c = 0; c < Tile<T, DP>::kSteps; ++c)
+    s = Mma<T>::mma(Tile<T, DP>::row_op(tile, row0 + (lane & 31), c, lane >> 5), f[c], s);
+  return s;
+}
+
+// both halves of the wave see both halves' values
+__device__ __forceinline__ float other_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(p) = v;
+  } else {
+    T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = from_f<T>(v[e]);
+    u32x2 u;
+    __builtin_memcpy(&u, t, 8);
+    *reinterpret_cast<u32x2*>(p) = u;
+  }
+}
+
+// a lane's column of the transposed result to its row in memory: 4 values a store
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* row, const f32x16 (&acc)[DP / 32], float by,
+                                              int half, int D) {
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * db + 8 * g + 4 * half;
+      if (d < D)
+        store4<T>(row + d, f32x4{acc[db][4 * g] * by, acc[db][4 * g + 1] * by,
+                                 acc[db][4 * g + 2] * by, acc[db][4 * g + 3] * by});
+    }
+}
+
+// Workgroups go to the 8 XCDs in turn; neighbours in `id` share keys and values, so each XCD gets
+// a contiguous share of the ids (its L2 then serves the re-reads).
+__device__ __forceinline__ unsigned xcd_id() {
+  const unsigned n = gridDim.x, x = blockIdx.x & 7, per = n >> 3, more = n & 7;
+  return x * per + min(x, more) + (blockIdx.x >> 3);
+}
+
+__device__ __forceinline__ int key_count(const Args& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
+}
+
+int64_t fwd_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV, int64_t D);
+int64_t bwd_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV);
+int check_problem(const char* what, int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                  int64_t KV, int64_t D, float scale, int64_t band);
+int read_strides3(const int64_t* s, int64_t L, int64_t H, int64_t D, int dtype, const void* base,
+                  int64_t* out, const char* name);
+int fwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st);
+int bwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st);
+
+}  // namespace attn
+}  // namespace smcv

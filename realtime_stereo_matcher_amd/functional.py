@@ -18,13 +18,20 @@ Reference operators mirrored (babiking/realtime_stereo_matcher):
   regression_presoftmax  model/mobile_stereo_net_v4.py:10-14
   hard_argmin/argmax     build-defined
   warp_by_flow_map       tools/warp.py:5-42, model/mobile_stereo_net_v2.py:59-96
+
+Matching by attention instead of a cost volume (no operator of the reference; differentiable):
+  rms_norm, rms_norm_e4m3         norm of the token stream, with the residual's addition
+  rotary, rotary_frequencies      rotary positions of queries and keys
+  cross_attention                 left tokens to the right view's, whose number may differ
 """
 from __future__ import annotations
 
+import math
 import numpy as np
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -584,3 +591,465 @@ def warp_by_flow_map(image, flow):
                                           _lib.strides_arg(flow), _ptr(ws) if ws is not None else None,
                                           nws, _stream(dev)), "sm_warp_by_flow_ws")
     return out if odt == torch.float32 else out.to(odt)
+
+
+# ------------------------------------------------------------------- matching by attention
+_TOKEN_DTYPES = {torch.float32: _lib.SM_F32, torch.float16: _lib.SM_F16, torch.bfloat16: _lib.SM_BF16}
+
+
+def _token_dtype(t, what, name):
+    code = _TOKEN_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype} of {name}; expected float32, float16 or "
+                        "bfloat16")
+    return code
+
+
+def _tensors(what, **named):
+    for name, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a tensor")
+
+
+def _token_ready(t):
+    """(tensor, its (batch, token, head) strides): unit stride of the values, the others and the
+    address multiples of 16 bytes -- a copy where they are not."""
+    per = 16 // t.element_size()
+    st = tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()))
+    if ((t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0
+            and st[0] % per == 0 and st[1] % per == 0 and st[2] % per == 0):
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:3]
+
+
+def _grads_wanted(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _attention_forward(q, k, v, lengths, mask, scale, band, want_lse):
+    b, lq, h, d = q.shape
+    lk, kv = k.shape[1], k.shape[2]
+    dev = q.device
+    with torch.cuda.device(dev):
+        out = torch.empty((b, lq, h, d), dtype=q.dtype, device=dev)
+        lse = torch.empty((b, kv, lq * (h // kv)) if kv else (b, 0, 0), dtype=torch.float32,
+                          device=dev) if want_lse else None
+        if out.numel():
+            lib = _lib.load()
+            q, qs = _token_ready(q)
+            k, ks = _token_ready(k)
+            v, vs = _token_ready(v)
+            nws = lib.sm_cross_attention_workspace_bytes(b, lq, lk, h, kv, d)
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+            _lib.check(lib.sm_cross_attention(
+                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse) if want_lse else None,
+                _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, _lib.int64s(*qs), _lib.int64s(*ks),
+                _lib.int64s(*vs), scale, band, None if lengths is None else _ptr(lengths),
+                None if mask is None else _ptr(mask), None if ws is None else _ptr(ws), nws,
+                _stream(dev)), "sm_cross_attention")
+    return out, lse
+
+
+def _attention_backward(q, k, v, out, lse, dout, lengths, mask, scale, band):
+    b, lq, h, d = q.shape
+    lk, kv = k.shape[1], k.shape[2]
+    dev = q.device
+    with torch.cuda.device(dev):
+        dq = torch.empty((b, lq, h, d), dtype=q.dtype, device=dev)
+        dk = torch.empty((b, lk, kv, d), dtype=q.dtype, device=dev)
+        dv = torch.empty_like(dk)
+        if dq.numel() or dk.numel():
+            lib = _lib.load()
+            q, qs = _token_ready(q)
+            k, ks = _token_ready(k)
+            v, vs = _token_ready(v)
+            dout, gs = _token_ready(dout)
+            nws = lib.sm_cross_attention_backward_workspace_bytes(b, lq, h, kv)
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+            _lib.check(lib.sm_cross_attention_backward(
+                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk),
+                _ptr(dv), _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, _lib.int64s(*qs),
+                _lib.int64s(*ks), _lib.int64s(*vs), _lib.int64s(*gs), scale, band,
+                None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask),
+                None if ws is None else _ptr(ws), nws, _stream(dev)), "sm_cross_attention_backward")
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask, scale, band):
+        out, lse = _attention_forward(q, k, v, lengths, mask, scale, band, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, mask)
+        ctx.scale, ctx.band = scale, band
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, out, lse, lengths, mask = ctx.saved_tensors
+        return (*_attention_backward(q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
+                None, None, None, None)
+
+
+def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_mask):
+    what = "cross_attention"
+    _tensors(what, query=query, key=key, value=value)
+    if query.dim() != 4 or key.dim() != 4:
+        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(query.shape)} and "
+                           f"{tuple(key.shape)}")
+    if key.shape != value.shape:
+        raise RuntimeError(f"{what}: key/value shape mismatch {tuple(key.shape)} vs {tuple(value.shape)}")
+    b, lq, h, d = query.shape
+    lk, kv = key.shape[1], key.shape[2]
+    if key.shape[0] != b or key.shape[3] != d:
+        raise RuntimeError(f"{what}: query {tuple(query.shape)} and key {tuple(key.shape)} differ in batch "
+                           "or head width")
+    if (h % kv if kv else h) != 0:
+        raise RuntimeError(f"{what}: {h} query heads are not a multiple of {kv} key heads")
+    if d % 8 != 0 or not 8 <= d <= 128:
+        raise RuntimeError(f"{what}: the head width must be a multiple of 8, 8 to 128, got {d}")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise RuntimeError(f"{what}: dtype mismatch {query.dtype}, {key.dtype}, {value.dtype}")
+    _token_dtype(query, what, "query")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3.4e38:
+        raise ValueError(f"{what}: the scale must be positive and finite, got {scale}")
+    band = 0
+    if max_disparity is not None:
+        band = int(max_disparity)
+        if not 1 <= band < 1 << 30:
+            raise ValueError(f"{what}: max_disparity must be positive, got {band}")
+    if key_lengths is not None:
+        _tensors(what, key_lengths=key_lengths)
+        if key_lengths.shape != (b,) or key_lengths.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"{what}: key_lengths must be {b} int32 or int64 values, got "
+                               f"{tuple(key_lengths.shape)} {key_lengths.dtype}")
+    if key_mask is not None:
+        _tensors(what, key_mask=key_mask)
+        if key_mask.shape != (b, lk) or key_mask.dtype != torch.bool:
+            raise RuntimeError(f"{what}: key_mask must be ({b}, {lk}) truth values, got "
+                               f"{tuple(key_mask.shape)} {key_mask.dtype}")
+    _device_check(*(t for t in (query, key, value, key_lengths, key_mask) if t is not None))
+    if key_lengths is not None:
+        if key_lengths.dtype == torch.int64:
+            key_lengths = key_lengths.clamp(0, lk).to(torch.int32)
+        key_lengths = key_lengths.contiguous()
+    if key_mask is not None:
+        key_mask = key_mask.contiguous()
+    return scale, band, key_lengths, key_mask
+
+
+def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengths=None,
+                    key_mask=None, return_lse=False):
+    """Attention of one view's tokens to another's: (B,Lq,H,D), (B,Lk,KV,D) x2 -> (B,Lq,H,D).
+
+    ``out[b,i,h] = sum_j p_ij value[b,j,kv]`` with ``p_i`` the softmax of ``scale * query[b,i,h] .
+    key[b,j,kv]`` over the allowed keys j, and ``kv = h // (H // KV)``: KV divides H, and query heads
+    share key heads.  ``scale``: D ** -0.5 by default.  Key j is allowed for token i where
+
+    - ``j < key_lengths[b]`` ((B,) int32 / int64, taken into 0 .. Lk): states padded to Lk,
+    - ``key_mask[b, j]`` ((B, Lk) bool): holes, e.g. invalid columns, and
+    - ``0 <= i - j < max_disparity``: the band of candidates of a cost volume's row.
+
+    A row without an allowed key gives 0.  Keys and values at positions past the length or masked are
+    never read, whatever they hold (NaN included); those inside have to be finite where the band
+    leaves them to some of 128 neighbouring rows only.  A row of a channels-last feature map is one sequence: ``feat.permute(0, 2, 3,
+    1).reshape(N * H, W, heads, C // heads)`` is a view, and with ``max_disparity`` the call is the
+    inner-product volume, its softmax over disparities and a weighted sum of values in one pass.
+
+    D is a multiple of 8 up to 128; any strides (a copy is made where the values are not contiguous
+    or rows not 16-byte aligned).  fp32, fp16 or bf16 with scores, statistics and sums in fp32; the
+    weights enter the second product rounded to the inputs' type.  Differentiable in query, key and
+    value, with the same bits on every run.  ``return_lse``: also the (B,Lq,H) fp32 logarithm of the
+    softmax's sum (-inf for an empty row; not differentiable), which joins parts of the keys.
+    """
+    if _traced():
+        out, lse = _ops().cross_attention(query, key, value, key_lengths, key_mask, scale, max_disparity)
+    else:
+        scale, band, lengths, mask = _attention_checks(query, key, value, scale, max_disparity,
+                                                       key_lengths, key_mask)
+        if _grads_wanted(query, key, value):
+            out, lse = _CrossAttention.apply(query, key, value, lengths, mask, scale, band)
+        else:
+            out, lse = _attention_forward(query, key, value, lengths, mask, scale, band, return_lse)
+    if not return_lse:
+        return out
+    b, lq, h, _ = query.shape
+    kv = key.shape[2]
+    lse = lse.view(b, kv, lq, h // kv).permute(0, 2, 1, 3).reshape(b, lq, h) if kv else lse.reshape(b, lq, 0)
+    return out, lse
+
+
+# ------------------------------------------------------------------------------ rotary positions
+def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None, low=1.0,
+                       high=32.0, device=None):
+    """The ``dim // 2`` frequencies (radians a position, float64) that ``rotary`` turns ``dim`` values
+    by: ``base ** (-2 n / dim)``, scaled for contexts ``factor`` times longer than was trained for:
+
+    - ``None``: not at all;
+    - ``"linear"``: all divided by ``factor`` (positions are interpolated);
+    - ``"base"``: of the larger base ``base * factor ** (dim / (dim - 2))``, which divides the lowest
+      by ``factor`` and leaves the highest;
+    - ``"parts"``: divided by ``factor`` where a pair makes fewer than ``low`` turns over
+      ``original_length`` positions, left where it makes more than ``high``, in between in proportion.
+    """
+    dim = int(dim)
+    if dim < 2 or dim % 2:
+        raise ValueError(f"rotary_frequencies: dim must be even and positive, got {dim}")
+    if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor > 0):
+        raise ValueError("rotary_frequencies: base and factor must be positive and finite")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError("rotary_frequencies: scaling must be None, 'linear', 'base' or 'parts'")
+    if scaling == "base":
+        if dim == 2:
+            raise ValueError("rotary_frequencies: 'base' needs more than one pair")
+        base = base * factor ** (dim / (dim - 2))
+    f = torch.tensor([base ** (-2.0 * n / dim) for n in range(dim // 2)], dtype=torch.float64)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        if original_length is None or original_length <= 0 or not 0 <= low < high:
+            raise ValueError("rotary_frequencies: 'parts' needs original_length > 0 and 0 <= low < high")
+        turns = original_length * f / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        f = f * (keep + (1 - keep) / factor)
+    return f.to(device) if device is not None else f
+
+
+def _rotary_run(x, positions, frequencies, interleaved, amplitude, inverse):
+    b, l, h, d = x.shape
+    dev = x.device
+    with torch.cuda.device(dev):
+        y = torch.empty((b, l, h, d), dtype=x.dtype, device=dev)
+        if y.numel():
+            if x.stride(3) != 1 and d > 1:
+                x = x.contiguous()
+            flags = ((_lib.SM_ROTARY_INTERLEAVED if interleaved else 0)
+                     | (_lib.SM_ROTARY_INVERSE if inverse else 0)
+                     | (_lib.SM_ROTARY_POS64 if positions.dtype == torch.int64 else 0))
+            st = (0 if n == 1 else s for n, s in zip(x.shape[:3], x.stride()))
+            ps = positions.stride(0) if positions.dim() == 2 and b > 1 else 0
+            _lib.check(_lib.load().sm_rotary(
+                _ptr(x), _ptr(positions), _ptr(frequencies), _ptr(y), _TOKEN_DTYPES[x.dtype], b, l, h,
+                d, 2 * frequencies.numel(), _lib.int64s(*st), ps, flags, amplitude, _stream(dev)),
+                "sm_rotary")
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, interleaved, amplitude):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = interleaved, amplitude
+        return _rotary_run(x, positions, frequencies, interleaved, amplitude, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return (_rotary_run(dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
+
+
+def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
+    """Rotary positions of (B,L,heads,D) tokens: the first ``2 * len(frequencies)`` values of every
+    head are turned in pairs by ``positions * frequencies`` radians, the others pass through.
+
+    ``positions``: (L,) or (B,L) int32 / int64; ``frequencies``: float64 on the tokens' device, kept by
+    the caller (``rotary_frequencies``).  ``layout``: ``"half"`` pairs value n with n + R/2,
+    ``"interleaved"`` 2n with 2n + 1.  ``amplitude`` multiplies the turned values.  The angle is formed
+    in 64 bits, so far positions are as exact as near ones; one rounding, to the tokens' type.
+    Differentiable in x.
+    """
+    if _traced():
+        return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
+    what = "rotary"
+    _tensors(what, x=x, positions=positions, frequencies=frequencies)
+    if x.dim() != 4:
+        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(x.shape)}")
+    _token_dtype(x, what, "x")
+    b, l, _, d = x.shape
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((l,), (b, l)):
+        raise RuntimeError(f"{what}: positions must be ({l},) or ({b}, {l}) int32 or int64, got "
+                           f"{tuple(positions.shape)} {positions.dtype}")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise RuntimeError(f"{what}: frequencies must be one row of float64, got "
+                           f"{tuple(frequencies.shape)} {frequencies.dtype}")
+    if not 2 <= 2 * frequencies.numel() <= d:
+        raise RuntimeError(f"{what}: {frequencies.numel()} pairs do not fit heads of {d} values")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"{what}: layout must be 'half' or 'interleaved'")
+    if frequencies.requires_grad:
+        raise RuntimeError(f"{what}: frequencies have no gradient")
+    _device_check(x, positions, frequencies)
+    if positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    frequencies = frequencies.contiguous()
+    how = layout == "interleaved", float(amplitude)
+    if _grads_wanted(x):
+        return _Rotary.apply(x, positions, frequencies, *how)
+    return _rotary_run(x, positions, frequencies, *how, False)
+
+
+# ------------------------------------------------------------------------------------- RMS norm
+def _rows(t, c):
+    """(the tensor as rows of c contiguous values, their stride)."""
+    t = t.reshape(-1, c)
+    if c > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else c
+
+
+def _norm_checks(what, x, weight, residual, eps):
+    _tensors(what, x=x, weight=weight, **({} if residual is None else {"residual": residual}))
+    if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
+        raise RuntimeError(f"{what}: expected (..., C) rows and (C,) weight, got {tuple(x.shape)} and "
+                           f"{tuple(weight.shape)}")
+    if not 1 <= x.shape[-1] <= 65536:
+        raise RuntimeError(f"{what}: rows of 1 to 65536 values, got {x.shape[-1]}")
+    _token_dtype(x, what, "x")
+    for name, t in (("weight", weight), ("residual", residual)):
+        if t is not None and t.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{what}: {name} must be {x.dtype} or float32, got {t.dtype}")
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"{what}: x/residual shape mismatch {tuple(x.shape)} vs {tuple(residual.shape)}")
+    if not 0.0 <= float(eps) < 3.4e38:
+        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    _device_check(x, weight, *(() if residual is None else (residual,)))
+
+
+def _norm_forward(x, weight, residual, eps, e4m3=None):
+    """(y, summed or None), or with ``e4m3`` (the group) (q, scales, summed or None)."""
+    dev, c = x.device, x.shape[-1]
+    shape, code = x.shape, _TOKEN_DTYPES[x.dtype]
+    with torch.cuda.device(dev):
+        summed = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+        y = torch.empty(shape, dtype=x.dtype if e4m3 is None else torch.float8_e4m3fn, device=dev)
+        scales = None
+        if e4m3 is not None:
+            per = (-(-c // e4m3),) if e4m3 else ()
+            scales = torch.empty((*shape[:-1], *per), dtype=torch.float32, device=dev)
+        if y.numel():
+            x, xs = _rows(x, c)
+            rcode, rs, rp, sp = code, c, None, None
+            if residual is not None:
+                residual, rs = _rows(residual, c)
+                rcode, rp, sp = _TOKEN_DTYPES[residual.dtype], _ptr(residual), _ptr(summed)
+            weight = weight.contiguous()
+            wcode = _TOKEN_DTYPES[weight.dtype]
+            lib = _lib.load()
+            if e4m3 is None:
+                _lib.check(lib.sm_rms_norm(_ptr(x), rp, _ptr(weight), _ptr(y), sp, code, rcode, wcode,
+                                           x.shape[0], c, xs, rs, eps, _stream(dev)), "sm_rms_norm")
+            else:
+                _lib.check(lib.sm_rms_norm_e4m3(
+                    _ptr(x), rp, _ptr(weight), _ptr(y), _ptr(scales), sp, code, rcode, wcode, x.shape[0],
+                    c, xs, rs, e4m3, eps, _stream(dev)), "sm_rms_norm_e4m3")
+    return (y, summed) if e4m3 is None else (y, scales, summed)
+
+
+def _norm_backward(summed, weight, dy, dsummed, dtype, eps):
+    """(dx, dresidual in summed's type or None where that is dx, dweight)."""
+    dev, c = summed.device, summed.shape[-1]
+    with torch.cuda.device(dev):
+        dx = torch.empty(summed.shape, dtype=dtype, device=dev)
+        dres = None if summed.dtype == dtype else torch.empty_like(dx, dtype=summed.dtype)
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+        n = summed.numel() // c
+        lib = _lib.load()
+        nws = lib.sm_rms_norm_backward_workspace_bytes(n, c)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        summed, ss = _rows(summed, c)
+        dy, ys = _rows(dy, c)
+        zs, zp = c, None
+        if dsummed is not None:
+            dsummed, zs = _rows(dsummed, c)
+            zp = _ptr(dsummed)
+        weight = weight.contiguous()
+        _lib.check(lib.sm_rms_norm_backward(
+            _ptr(summed), _ptr(weight), _ptr(dy), zp, _ptr(dx), None if dres is None else _ptr(dres),
+            _ptr(dw), _TOKEN_DTYPES[dtype], _TOKEN_DTYPES[summed.dtype], _TOKEN_DTYPES[weight.dtype], n,
+            c, ss, ys, zs, eps, None if ws is None else _ptr(ws), nws, _stream(dev)),
+            "sm_rms_norm_backward")
+    return dx, dres, dw
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        return _norm_forward(x, weight, None, eps)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        dx, _, dw = _norm_backward(x, weight, dy, None, x.dtype, ctx.eps)
+        return dx, dw, None
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, summed = _norm_forward(x, weight, residual, eps)
+        ctx.save_for_backward(summed, weight)
+        ctx.eps, ctx.dtype = eps, x.dtype
+        ctx.set_materialize_grads(False)
+        return y, summed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dsummed):
+        summed, weight = ctx.saved_tensors
+        if dy is None:  # only the stream was used
+            if dsummed is None:
+                return None, None, None, None
+            return dsummed.to(ctx.dtype), None, dsummed, None
+        dx, dres, dw = _norm_backward(summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
+        return dx, dw, dx if dres is None else dres, None
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """Root-mean-square norm of (..., C) rows: ``y = s / sqrt(mean(s^2) + eps) * weight``.
+
+    Without a residual ``s = x`` and y is returned.  With one ``s = x + residual``, rounded to the
+    residual's type, and ``(y, s)`` is returned: s is the stream that the next layer adds to, and y is
+    the norm of s as it is handed on.  x is fp32, fp16 or bf16, y has its type; weight (C,) and
+    residual have it or are fp32 (a 32-bit stream beside 16-bit layers).  C is 1 to 65536; sums are
+    fp32.  Differentiable in x, weight and residual (weight's gradient is summed in one order).
+    """
+    if _traced():
+        if residual is None:
+            return _ops().rms_norm(x, weight, float(eps))
+        return _ops().add_rms_norm(x, weight, residual, float(eps))
+    _norm_checks("rms_norm", x, weight, residual, eps)
+    eps = float(eps)
+    if residual is None:
+        if _grads_wanted(x, weight):
+            return _RmsNorm.apply(x, weight, eps)
+        return _norm_forward(x, weight, None, eps)[0]
+    if _grads_wanted(x, weight, residual):
+        return _AddRmsNorm.apply(x, weight, residual, eps)
+    return _norm_forward(x, weight, residual, eps)
+
+
+def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
+    """``rms_norm`` with y in 8 bits, for a product that takes them: ``(q, scales)``, or ``(q, scales,
+    s)`` with a residual, where ``y ~ q * scales``.
+
+    q is (..., C) float8_e4m3fn, rounded to nearest from the fp32 y / scale; a scale is max|y| / 448
+    over the row (``group=None``; scales (...)) or over each 128 values of it (``group=128``; scales
+    (..., ceil(C / 128))), and 1 where y is 0.  Forward only.
+    """
+    if group not in (None, 128):
+        raise ValueError(f"rms_norm_e4m3: group must be None (a row) or 128, got {group}")
+    if _traced():
+        if residual is None:
+            return _ops().rms_norm_e4m3(x, weight, float(eps), group or 0)
+        return _ops().add_rms_norm_e4m3(x, weight, residual, float(eps), group or 0)
+    _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
+    if _grads_wanted(x, weight, residual):
+        raise NotImplementedError("rms_norm_e4m3 is forward only: call it under torch.no_grad()")
+    out = _norm_forward(x, weight, residual, float(eps), group or 0)
+    return out[:2] if residual is None else out

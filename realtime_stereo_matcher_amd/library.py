@@ -7,12 +7,14 @@ not see through it.  Registered here with ``torch.library.custom_op``, each oper
 of the traced graph: ``functional`` routes a call through ``torch.ops.stereocv.<name>`` whenever
 it runs under ``torch.jit.trace`` or a compiler (dynamo / export), the fake kernel gives
 FakeTensor tracing the output's shape, dtype and device, and the real kernel is the same
-libstereocv call as the eager path (no CPU fallback).  The ops are forward-only like the rest
-of the engine: their backward raises ``NotImplementedError``.
+libstereocv call as the eager path (no CPU fallback).  The cost-volume ops are forward-only like
+the rest of that engine: their backward raises ``NotImplementedError``.  The matching-transformer
+ops have their gradients, as ops of their own.
 """
 from __future__ import annotations
 
 import threading
+from typing import Optional
 
 import torch
 
@@ -250,3 +252,186 @@ inner_product_soft_argmin_novolume = _register("inner_product_soft_argmin_novolu
                                                _fused_novolume, _fused_novolume_fake)
 warp_by_flow_map = _register("warp_by_flow_map", _warp, _warp_fake)
 v4_volume = _register("v4_volume", _v4, _v4_fake)
+
+
+# ----------------------------------------------------------------- matching by attention
+def _register_with_grad(name, impl, fake, setup, backward):
+    op = torch.library.custom_op(f"stereocv::{name}", mutates_args=())(impl)
+    op.register_fake(fake)
+    torch.library.register_autograd(f"stereocv::{name}", backward, setup_context=setup)
+    return op
+
+
+def _attn(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+          key_lengths: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
+          scale: Optional[float] = None,
+          max_disparity: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
+                                                     key_lengths, key_mask)
+    return F._attention_forward(query, key, value, lengths, mask, scale, band, True)
+
+
+def _attn_fake(query, key, value, key_lengths=None, key_mask=None, scale=None, max_disparity=None):
+    b, lq, h, _ = query.shape
+    kv = key.shape[2]
+    return (_empty(query.shape, query),
+            _empty((b, kv, lq * (h // kv)) if kv else (b, 0, 0), query, torch.float32))
+
+
+def _attn_setup(ctx, inputs, output):
+    q, k, v, lengths, mask, scale, max_disparity = inputs
+    ctx.save_for_backward(q, k, v, *output, lengths, mask)
+    ctx.scale, ctx.max_disparity = scale, max_disparity
+
+
+def _attn_grad(ctx, dout, dlse):
+    q, k, v, out, lse, lengths, mask = ctx.saved_tensors
+    dq, dk, dv = torch.ops.stereocv.cross_attention_backward(
+        q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.max_disparity)
+    return dq, dk, dv, None, None, None, None
+
+
+def _attn_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, out: torch.Tensor,
+                   lse: torch.Tensor, dout: torch.Tensor,
+                   key_lengths: Optional[torch.Tensor] = None,
+                   key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   max_disparity: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
+                                                     key_lengths, key_mask)
+    if out.shape != query.shape or dout.shape != query.shape or out.dtype != query.dtype \
+            or dout.dtype != query.dtype or not out.is_contiguous():
+        raise RuntimeError("cross_attention_backward: out and dout must have the query's shape and "
+                           "type, and out must be contiguous")
+    kv = key.shape[2]
+    rows = query.shape[1] * (query.shape[2] // kv if kv else 0)
+    if tuple(lse.shape) != (query.shape[0], kv, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise RuntimeError("cross_attention_backward: lse must be the forward call's")
+    F._device_check(query, out, lse, dout)
+    return F._attention_backward(query, key, value, out, lse, dout, lengths, mask, scale, band)
+
+
+def _attn_backward_fake(query, key, value, out, lse, dout, key_lengths=None, key_mask=None, scale=None,
+                        max_disparity=None):
+    return _empty(query.shape, query), _empty(key.shape, key), _empty(key.shape, key)
+
+
+def _rot(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half",
+         amplitude: float = 1.0, inverse: bool = False) -> torch.Tensor:
+    with _Inside(), torch.no_grad():
+        if not inverse:
+            return F.rotary(x, positions, frequencies, layout, amplitude)
+        return F._rotary_run(x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
+                             amplitude, True)
+
+
+def _rot_fake(x, positions, frequencies, layout="half", amplitude=1.0, inverse=False):
+    return _empty(x.shape, x)
+
+
+def _rot_setup(ctx, inputs, output):
+    _, positions, frequencies, ctx.layout, ctx.amplitude, ctx.inverse = inputs
+    ctx.save_for_backward(positions, frequencies)
+
+
+def _rot_grad(ctx, dy):
+    positions, frequencies = ctx.saved_tensors
+    dx = torch.ops.stereocv.rotary(dy, positions, frequencies, ctx.layout, ctx.amplitude, not ctx.inverse)
+    return dx, None, None, None, None, None
+
+
+def _norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    with _Inside(), torch.no_grad():
+        return F.rms_norm(x, weight, None, eps)
+
+
+def _norm_fake(x, weight, eps=1e-6):
+    return _empty(x.shape, x)
+
+
+def _norm_setup(ctx, inputs, output):
+    x, weight, ctx.eps = inputs
+    ctx.save_for_backward(x, weight)
+
+
+def _norm_grad(ctx, dy):
+    x, weight = ctx.saved_tensors
+    dx, _, dw = torch.ops.stereocv.rms_norm_backward(x, weight, dy, None, ctx.eps)
+    return dx, dw, None
+
+
+def _add_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor,
+              eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    with _Inside(), torch.no_grad():
+        return F.rms_norm(x, weight, residual, eps)
+
+
+def _add_norm_fake(x, weight, residual, eps=1e-6):
+    return _empty(x.shape, x), _empty(x.shape, residual)
+
+
+def _add_norm_setup(ctx, inputs, output):
+    x, weight, _, ctx.eps = inputs
+    ctx.save_for_backward(output[1], weight)
+
+
+def _add_norm_grad(ctx, dy, dsummed):
+    summed, weight = ctx.saved_tensors
+    dx, dres, dw = torch.ops.stereocv.rms_norm_backward(summed, weight, dy, dsummed, ctx.eps)
+    return dx, dw, dx if summed.dtype == dy.dtype else dres, None
+
+
+def _norm_backward(summed: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor,
+                   dsummed: Optional[torch.Tensor] = None,
+                   eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    F._norm_checks("rms_norm_backward", dy, weight, summed, eps)
+    if dsummed is not None and (dsummed.shape != summed.shape or dsummed.dtype != summed.dtype):
+        raise RuntimeError("rms_norm_backward: dsummed must have summed's shape and type")
+    dx, dres, dw = F._norm_backward(summed, weight, dy, dsummed, dy.dtype, eps)
+    return dx, dx.new_empty(0, dtype=summed.dtype) if dres is None else dres, dw
+
+
+def _norm_backward_fake(summed, weight, dy, dsummed=None, eps=1e-6):
+    same = summed.dtype == dy.dtype
+    return (_empty(dy.shape, dy), _empty((0,) if same else summed.shape, summed),
+            _empty(weight.shape, weight))
+
+
+def _norm8_shape(x, group):
+    return (*x.shape[:-1], -(-x.shape[-1] // group)) if group else x.shape[:-1]
+
+
+def _norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+           group: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    with _Inside(), torch.no_grad():
+        return F.rms_norm_e4m3(x, weight, None, eps, group or None)
+
+
+def _norm8_fake(x, weight, eps=1e-6, group=0):
+    return _empty(x.shape, x, torch.float8_e4m3fn), _empty(_norm8_shape(x, group), x, torch.float32)
+
+
+def _add_norm8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor, eps: float = 1e-6,
+               group: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    with _Inside(), torch.no_grad():
+        return F.rms_norm_e4m3(x, weight, residual, eps, group or None)
+
+
+def _add_norm8_fake(x, weight, residual, eps=1e-6, group=0):
+    return (*_norm8_fake(x, weight, eps, group), _empty(x.shape, residual))
+
+
+def _plain_op(name, impl, fake):
+    op = torch.library.custom_op(f"stereocv::{name}", mutates_args=())(impl)
+    op.register_fake(fake)
+    return op
+
+
+cross_attention = _register_with_grad("cross_attention", _attn, _attn_fake, _attn_setup, _attn_grad)
+cross_attention_backward = _plain_op("cross_attention_backward", _attn_backward, _attn_backward_fake)
+rotary = _register_with_grad("rotary", _rot, _rot_fake, _rot_setup, _rot_grad)
+rms_norm = _register_with_grad("rms_norm", _norm, _norm_fake, _norm_setup, _norm_grad)
+add_rms_norm = _register_with_grad("add_rms_norm", _add_norm, _add_norm_fake, _add_norm_setup,
+                                   _add_norm_grad)
+rms_norm_backward = _plain_op("rms_norm_backward", _norm_backward, _norm_backward_fake)
+rms_norm_e4m3 = _register("rms_norm_e4m3", _norm8, _norm8_fake)
+add_rms_norm_e4m3 = _register("add_rms_norm_e4m3", _add_norm8, _add_norm8_fake)
