@@ -318,7 +318,7 @@ int sm_rms_norm(const void* x, const void* residual, const void* weight, void* y
                 int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
                 int64_t x_stride, int64_t residual_stride, float eps, void* stream);
 /* The same with y in 8 bits: q = e4m3(y / scale), scale = max |y| / 448 over the row (group 0;
- * scales (rows)) or over each 128 values (group 128; scales (rows, ceil(C / 128))); 1 where y is 0. */
+ * scales (rows, 1)) or over each 128 values (group 128; scales (rows, ceil(C / 128))); 1 where y is 0. */
 int sm_rms_norm_e4m3(const void* x, const void* residual, const void* weight, void* q, float* scales,
                      void* summed, int dtype, int residual_dtype, int weight_dtype, int64_t rows,
                      int64_t C, int64_t x_stride, int64_t residual_stride, int64_t group, float eps,

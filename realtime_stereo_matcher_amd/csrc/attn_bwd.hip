@@ -6,7 +6,12 @@
 // that every sum has one owner: no atomics, the same bits on every run, and the gradients of key
 // heads shared by several query heads are summed in the owner's registers.  That forms the scores
 // and their gradient twice (7 products where one kernel with atomic sums would have 5).
-//   attn_dq   a wave owns 32 query rows; writes dq, and per row delta and the logarithm in base 2
+//   attn_dq   a wave owns 32 query rows; writes dq, and per row delta and the logarithm in base 2.
+//             In 16 bits g . o carries the rounding of o and of the weights that formed it, which
+//             shifts a whole row of ds.  So the row's delta = sum_j p_ij (g_i . v_j) is summed in
+//             fp32 beside the products: attn_dkv takes that one, and dq, formed with g . o, is put
+//             right at the end by the difference times sum_j p_ij k_j (one product more, on the
+//             keys already read).
 //   attn_dkv  a wave owns 32 keys; loops over the rows of all heads that share them
 // fp16: ds would fall out of the type's range for small gradients, so g enters with a power of
 // two: one that brings the row's largest |g| into [1/2, 1) in attn_dq (a lane's scalar), the
@@ -93,7 +98,7 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
   if (half == 0) {
     a.row_lse[at] = lse2;
-    a.row_delta[at] = delta;
+    if constexpr (sizeof(T) == 4) a.row_delta[at] = delta;
   }
   int shift = 0;
   if constexpr (kScaled) {
@@ -135,11 +140,16 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     TL::template load<KT, 256>(V, a.vs[1], t * KT, dst + C::kTileBytes, tid, a.D, ok);
   };
 
-  f32x16 dq[DP / 32];
+  // dq, and (16-bit types) the weighted mean of the keys
+  constexpr int N = sizeof(T) == 4 ? 1 : 2;
+  f32x16 dq[N][DP / 32];
+  float sum = 0.f;  // of p (g . v): delta again
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dq[db][r] = 0.f;
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
 
   uint64_t bits = 0;
   int byte = 0;
@@ -170,7 +180,8 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 s = mma_rows<T, DP>(kt, 32 * kb, q, lane);
-      f32x16 ds = mma_rows<T, DP>(vt, 32 * kb, g, lane);
+      f32x16 ds[N];  // and the weights
+      ds[0] = mma_rows<T, DP>(vt, 32 * kb, g, lane);
       if (seen != kAll) {
         const unsigned w = (unsigned)(seen >> (32 * kb)) >> (4 * half);
 #pragma unroll
@@ -184,13 +195,28 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
           s[r] = (unsigned)(d - (8 * (r >> 2) + (r & 3))) < (unsigned)a.band ? s[r] : -INFINITY;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * (ds[r] - delta);
-      mma_transposed<T, DP>(dq, kt, 32 * kb, ds, lane);
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));
+        if constexpr (N == 2) {
+          sum = fmaf(p, ds[0][r], sum);
+          ds[1][r] = p;
+        }
+        ds[0][r] = p * (ds[0][r] - delta);
+      }
+      mma_transposed<T, DP, N>(dq, kt, 32 * kb, ds, lane);
     }
   }
+  if constexpr (N == 2) {
+    sum = other_half_sum(sum);
+    if (half == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift);
+    delta -= sum;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(delta, dq[1][db][r], dq[0][db][r]);
+  }
   if (!there) return;
-  store_columns<T, DP>(static_cast<T*>(a.dq) + orow, dq, __builtin_ldexpf(a.scale, -shift), half, a.D);
+  store_columns<T, DP>(static_cast<T*>(a.dq) + orow, dq[0], __builtin_ldexpf(a.scale, -shift), half, a.D);
 }
 
 template <typename T, int DP, bool KMASK>

@@ -165,11 +165,12 @@ template <typename T, int DP> struct Tile {
 // registers of a block that hold 4 (fp32) or 8 (16-bit) consecutive contraction steps
 __device__ __forceinline__ int crow(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
-// acc[db] += (tile rows row0 .. row0+31, transposed) * block, where `block` holds a 32x32 result
-// (tile rows x lane columns): values of the tile's column are the rows of the product.
-template <typename T, int DP>
-__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned tile, int row0,
-                                               const f32x16& block, int lane) {
+// acc[n][db] += (tile rows row0 .. row0+31, transposed) * block[n], where a block holds a 32x32
+// result (tile rows x lane columns): values of the tile's column are the rows of the product.  N
+// products share the reads of the tile.
+template <typename T, int DP, int N>
+__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[N][DP / 32], unsigned tile, int row0,
+                                               const f32x16 (&block)[N], int lane) {
   using TL = Tile<T, DP>;
   if constexpr (sizeof(T) == 4) {
     const int half = lane >> 5, col = lane & 31;
@@ -180,7 +181,9 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned 
       for (int db = 0; db < DP / 32; ++db) {
         const int ch = (8 * db + (col >> 2)) ^ TL::twist(row);
         const float a = lds_get<float>(tile + row * TL::kRowBytes + ch * 16 + (col & 3) * 4);
-        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, block[r], acc[db], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, block[n][r], acc[n][db], 0, 0, 0);
       }
     }
   } else {
@@ -189,9 +192,11 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned 
     const int half = lane >> 5, g = (lane >> 4) & 1, l16 = lane & 15;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      Frag<T> p;
+      Frag<T> p[N];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) Mma<T>::put(p, e, block[8 * s + e]);
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) Mma<T>::put(p[n], e, block[n][8 * s + e]);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) {
         s16x4 lo, hi;
@@ -204,7 +209,9 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned 
             reinterpret_cast<lds_s4*>(at + 8 * TL::kRowBytes));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[db] = Mma<T>::mma(__builtin_bit_cast(Frag<T>, both), p, acc[db]);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n][db] = Mma<T>::mma(__builtin_bit_cast(Frag<T>, both), p[n], acc[n][db]);
       }
     }
   }
@@ -212,6 +219,13 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned 
 
 // a row in registers, as the right operand of all steps over its values
 template <typename T, int DP> using RowOps = Frag<T>[Tile<T, DP>::kSteps];
+
+template <typename T, int DP>
+__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned tile, int row0,
+                                               const f32x16& block, int lane) {
+  mma_transposed<T, DP, 1>(reinterpret_cast<f32x16(&)[1][DP / 32]>(acc), tile, row0,
+                           reinterpret_cast<const f32x16(&)[1]>(block), lane);
+}
 
 // right operand of one row (a query or a key) a lane, straight from global memory
 template <typename T, int DP>

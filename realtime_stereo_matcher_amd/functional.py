@@ -927,8 +927,8 @@ def _norm_forward(x, weight, residual, eps, e4m3=None):
         y = torch.empty(shape, dtype=x.dtype if e4m3 is None else torch.float8_e4m3fn, device=dev)
         scales = None
         if e4m3 is not None:
-            per = (-(-c // e4m3),) if e4m3 else ()
-            scales = torch.empty((*shape[:-1], *per), dtype=torch.float32, device=dev)
+            per = -(-c // e4m3) if e4m3 else 1
+            scales = torch.empty((*shape[:-1], per), dtype=torch.float32, device=dev)
         if y.numel():
             x, xs = _rows(x, c)
             rcode, rs, rp, sp = code, c, None, None
@@ -1039,7 +1039,7 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
     s)`` with a residual, where ``y ~ q * scales``.
 
     q is (..., C) float8_e4m3fn, rounded to nearest from the fp32 y / scale; a scale is max|y| / 448
-    over the row (``group=None``; scales (...)) or over each 128 values of it (``group=128``; scales
+    over the row (``group=None``; scales (..., 1)) or over each 128 values of it (``group=128``; scales
     (..., ceil(C / 128))), and 1 where y is 0.  Forward only.
     """
     if group not in (None, 128):

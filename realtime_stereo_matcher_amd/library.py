@@ -397,7 +397,7 @@ def _norm_backward_fake(summed, weight, dy, dsummed=None, eps=1e-6):
 
 
 def _norm8_shape(x, group):
-    return (*x.shape[:-1], -(-x.shape[-1] // group)) if group else x.shape[:-1]
+    return (*x.shape[:-1], -(-x.shape[-1] // group) if group else 1)
 
 
 def _norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,

@@ -777,7 +777,7 @@ def test_matching_ops_fake():
         assert y.dtype == torch.half and s.dtype == torch.float32
         q8, sc = ops.rms_norm_e4m3(x, w, 1e-6, 128)
         assert q8.dtype == torch.float8_e4m3fn and sc.shape == (3, 2)
-        assert ops.add_rms_norm_e4m3(x, w, r)[1].shape == (3,)
+        assert ops.add_rms_norm_e4m3(x, w, r)[1].shape == (3, 1)
         dx, dr, dw = ops.rms_norm_backward(r, w, x)
         assert dx.dtype == torch.half and dr.shape == r.shape and dw.shape == w.shape
 
