@@ -272,8 +272,8 @@ int sm_v4_volume(const void* featL, const void* featR, void* out, int dtype,
  * A row without an allowed key gives 0 (and -inf in lse).  What keys and values hold at positions
  * past the length or masked is not read.  lse: NULL or (B, KV, Lq * H / KV) float32, the natural
  * logarithm of the softmax's sum, row i * (H / KV) + h % (H / KV): what the backward call needs.
- * Strides: element strides of (batch, token, head), multiples of 16 bytes (NULL: contiguous);
- * pointers 16-byte aligned.  The workspace (16-byte aligned; 0 bytes: none is used) holds partial
+ * Strides: element strides of (batch, token, head), multiples of 16 bytes (NULL: contiguous), tokens
+ * less than 2^24 bytes apart; pointers 16-byte aligned.  The workspace (16-byte aligned; 0 bytes: none is used) holds partial
  * results when few rows attend to many keys. */
 int64_t sm_cross_attention_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV,
                                            int64_t D);

@@ -368,9 +368,9 @@ int attention_args(attn::Args* a, const char* what, const void* query, const voi
                    const int64_t* v_strides, float scale, int64_t max_disparity,
                    const int32_t* key_lengths, const uint8_t* key_mask) {
   if (const int rc = attn::check_problem(what, dtype, B, Lq, Lk, H, KV, D, scale, max_disparity)) return rc;
-  if (const int rc = attn::read_strides3(q_strides, Lq, H, D, dtype, query, a->qs, "query")) return rc;
-  if (const int rc = attn::read_strides3(k_strides, Lk, KV, D, dtype, key, a->ks, "key")) return rc;
-  if (const int rc = attn::read_strides3(v_strides, Lk, KV, D, dtype, value, a->vs, "value")) return rc;
+  if (const int rc = attn::read_strides3(q_strides, Lq, H, D, dtype, query, a->qs, 0, "query")) return rc;
+  if (const int rc = attn::read_strides3(k_strides, Lk, KV, D, dtype, key, a->ks, 1, "key")) return rc;
+  if (const int rc = attn::read_strides3(v_strides, Lk, KV, D, dtype, value, a->vs, 1, "value")) return rc;
   if (B * Lq * H > 0 && !query) return fail(SM_EINVAL, std::string(what) + ": null query pointer");
   if (B * Lk * KV > 0 && (!key || !value))
     return fail(SM_EINVAL, std::string(what) + ": null key or value pointer");
@@ -438,7 +438,8 @@ extern "C" int sm_cross_attention_backward(
   if (const int rc = attention_args(&a, "cross_attention_backward", query, key, value, dtype, B, Lq, Lk,
                                     H, KV, D, q_strides, k_strides, v_strides, scale, max_disparity,
                                     key_lengths, key_mask)) return rc;
-  if (const int rc = attn::read_strides3(dout_strides, Lq, H, D, dtype, dout, a.gs, "dout")) return rc;
+  if (const int rc = attn::read_strides3(dout_strides, Lq, H, D, dtype, dout, a.gs, a.G, "dout")) return rc;
+  if (const int rc = attn::read_strides3(q_strides, Lq, H, D, dtype, query, a.qs, a.G, "query")) return rc;
   if (workspace_bytes < 0) return fail(SM_EINVAL, "cross_attention_backward: negative workspace size");
   const bool rows = B * Lq * H > 0, keys = B * Lk * KV > 0;
   if ((rows && (!out || !lse || !dout || !dquery)) || (keys && (!dkey || !dvalue)))

@@ -44,7 +44,6 @@ template <typename T, int DP, bool KMASK>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dq(Args a) {
   using C = BCfg<T, DP>;
   using TL = Tile<T, DP>;
-  using frag = Frag<T>;
   constexpr int KT = C::kTile, KB = KT / 32;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -59,26 +58,17 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   const int token = row / a.G, head = kv * a.G + row % a.G;
   const bool there = row < a.rows;
 
-  const int keys = key_count(a, b);
-  int jlo = 0, jhi = keys;
-  if (a.band > 0) {
-    const int last = min(wg_row0 + kRows, a.rows) - 1;
-    jlo = max(0, wg_row0 / a.G - a.band + 1);
-    jhi = min(keys, last / a.G + 1);
-  }
-  const int tb = jlo / KT, te = jhi > jlo ? (jhi + KT - 1) / KT : tb;
+  Keys<KT, KMASK> keys(a, b, wg_row0, kRows);
 
-  const T* K = static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2];
-  const T* V = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
   const int64_t orow = (((int64_t)b * a.Lq + token) * a.H + head) * a.D;
-  frag q[TL::kSteps], g[TL::kSteps];
+  RowOps<T, DP> q, g;
   load_rows<T, DP>(q, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)token * a.qs[1] +
                           head * a.qs[2], there, half, a.D);
   load_rows<T, DP>(g, static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)token * a.gs[1] +
                           head * a.gs[2], there, half, a.D);
   float delta = 0.f, most = 0.f;
   {
-    frag o[TL::kSteps];
+    RowOps<T, DP> o;
     load_rows<T, DP>(o, static_cast<const T*>(a.o) + orow, there, half, a.D);
 #pragma unroll
     for (int s = 0; s < TL::kSteps; ++s)
@@ -124,20 +114,23 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   }
 
   const unsigned lds = lds_addr(smem);
-  const uint8_t* mask = KMASK ? a.mask + (int64_t)b * a.Lk : nullptr;
-  auto mask_byte = [&](int t) -> int {
-    const int j = t * KT + lane;
-    return lane < KT && t < te && j < keys ? mask[j] : 0;
-  };
-  auto length_bits = [&](int t) -> uint64_t {
-    const int n = keys - t * KT;
-    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
-  };
-  constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
+  const Reads<T, DP> from(lds, lane);
+  const int wave0 = wave * 64;
+  const unsigned kb_row = (unsigned)a.ks[1] * sizeof(T), vb_row = (unsigned)a.vs[1] * sizeof(T);
+  Stage<T, DP, KT, 256> sk, sv;
+  sk.init(tid, a.D, [&](int r) { return r * kb_row; });
+  sv.init(tid, a.D, [&](int r) { return r * vb_row; });
+  const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
+  const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
-    auto ok = [&](int, int r) { return ((bits >> r) & 1) != 0; };
-    TL::template load<KT, 256>(K, a.ks[1], t * KT, dst, tid, a.D, ok);
-    TL::template load<KT, 256>(V, a.vs[1], t * KT, dst + C::kTileBytes, tid, a.D, ok);
+    const uint64_t kp = K + (uint64_t)t * KT * kb_row, vp = V + (uint64_t)t * KT * vb_row;
+    if (bits == keys.kAll) {
+      sk.copy(kp, dst, wave0);
+      sv.copy(vp, dst + C::kTileBytes, wave0);
+    } else if (bits != 0) {
+      sk.copy(kp, dst, wave0, tid, bits, kb_row);
+      sv.copy(vp, dst + C::kTileBytes, wave0, tid, bits, vb_row);
+    }
   };
 
   // dq, and (16-bit types) the weighted mean of the keys
@@ -151,49 +144,40 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
 
+  int t = keys.tb;
   uint64_t bits = 0;
   int byte = 0;
-  if (tb < te) {
-    bits = KMASK ? __ballot(mask_byte(tb)) : length_bits(tb);
-    if (KMASK) byte = mask_byte(tb + 1);
-    copy(tb, lds, bits);
+  if (t < keys.te) {
+    bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
+    copy(t, lds, bits);
   }
-  for (int t = tb, buf = 0; t < te; ++t, buf ^= 1) {
+  if (KMASK) byte = keys.byte(t + 1, lane);
+  auto step = [&](auto buf) {
+    constexpr int kBuf = decltype(buf)::value * 2 * C::kTileBytes;
     publish();
     uint64_t next = 0;
-    if (t + 1 < te) {
-      next = KMASK ? __ballot(byte) : length_bits(t + 1);
-      if (KMASK) byte = mask_byte(t + 2);
-      copy(t + 1, lds + (buf ^ 1) * 2 * C::kTileBytes, next);
+    if (t + 1 < keys.te) {
+      next = KMASK ? __ballot(byte) : keys.by_length(t + 1);
+      if (KMASK) byte = keys.byte(t + 2, lane);
+      copy(t + 1, lds + (2 * C::kTileBytes - kBuf), next);
     }
-    const unsigned kt = lds + buf * 2 * C::kTileBytes, vt = kt + C::kTileBytes;
-    const uint64_t seen = bits & kAll;
+    const uint64_t seen = bits;
     bits = next;
+    if (seen == 0) return;
     bool edge = false;
     if (a.band > 0) {
       const int j0 = t * KT, j1 = j0 + KT - 1;
       const int i0 = row0 / a.G, i1 = min(row0 + 31, a.rows - 1) / a.G;
-      if (j0 > i1 || j1 <= i0 - a.band) continue;
+      if (j0 > i1 || j1 <= i0 - a.band) return;
       edge = j1 > i0 || j0 <= i1 - a.band;
     }
-    if (seen == 0) continue;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      f32x16 s = mma_rows<T, DP>(kt, 32 * kb, q, lane);
+      f32x16 s = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
       f32x16 ds[N];  // and the weights
-      ds[0] = mma_rows<T, DP>(vt, 32 * kb, g, lane);
-      if (seen != kAll) {
-        const unsigned w = (unsigned)(seen >> (32 * kb)) >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
-      }
-      if (edge) {
-        const int d = token - (t * KT + 32 * kb + 4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = (unsigned)(d - (8 * (r >> 2) + (r & 3))) < (unsigned)a.band ? s[r] : -INFINITY;
-      }
+      ds[0] = mma_rows<T, DP>(from, kBuf + C::kTileBytes, 32 * kb, g);
+      if (seen != keys.kAll) mask_block(s, (unsigned)(seen >> (32 * kb)), half);
+      if (edge) band_block(s, token - (t * KT + 32 * kb), a.band, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));
@@ -203,8 +187,14 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
         }
         ds[0][r] = p * (ds[0][r] - delta);
       }
-      mma_transposed<T, DP, N>(dq, kt, 32 * kb, ds, lane);
+      mma_transposed<T, DP, N>(dq, from, kBuf, 32 * kb, ds);
     }
+  };
+  while (t < keys.te) {
+    step(std::integral_constant<int, 0>{});
+    if (++t >= keys.te) break;
+    step(std::integral_constant<int, 1>{});
+    ++t;
   }
   if constexpr (N == 2) {
     sum = other_half_sum(sum);
@@ -222,8 +212,6 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 template <typename T, int DP, bool KMASK>
 __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dkv(Args a) {
   using C = BCfg<T, DP>;
-  using TL = Tile<T, DP>;
-  using frag = Frag<T>;
   constexpr int RT = C::kTile, RB = RT / 32;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   constexpr float kUp = kScaled ? 14.f : 0.f;
@@ -237,10 +225,10 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   id /= key_tiles;
   const int kv = id % a.KV, b = id / a.KV;
   const int wg_j0 = jt * kRows, j0 = wg_j0 + 32 * wave, j = j0 + (lane & 31);
-  const int keys = key_count(a, b);
+  const int keys = a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
   const bool there = j < keys && (!KMASK || a.mask[(int64_t)b * a.Lk + min(j, a.Lk - 1)] != 0);
 
-  frag k[TL::kSteps], v[TL::kSteps];
+  RowOps<T, DP> k, v;
   load_rows<T, DP>(k, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)j * a.ks[1] +
                           kv * a.ks[2], there, half, a.D);
   load_rows<T, DP>(v, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)j * a.vs[1] +
@@ -269,30 +257,40 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   }
 
   const unsigned lds = lds_addr(smem);
-  const T* Q = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)kv * a.G * a.qs[2];
-  const T* GO = static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)kv * a.G * a.gs[2];
+  const Reads<T, DP> from(lds, lane);
+  const int wave0 = wave * 64;
+  const uint64_t Q = reinterpret_cast<uint64_t>(static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)kv * a.G * a.qs[2]);
+  const uint64_t GO = reinterpret_cast<uint64_t>(static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)kv * a.G * a.gs[2]);
+  // Row t RT + r is token (t RT + r) / G: where G divides RT the offsets from the tile's first token
+  // are the same in every tile.
+  const bool regular = RT % a.G == 0;
+  auto row_at = [&](int row, int token0, const int64_t* st) -> unsigned {
+    const int token = row / a.G, g = row - token * a.G;
+    return ((token - token0) * (unsigned)st[1] + g * (unsigned)st[2]) * (unsigned)sizeof(T);
+  };
+  Stage<T, DP, RT, 256> sq, sg;
+  sq.init(tid, a.D, [&](int r) { return row_at(r, 0, a.qs); });
+  sg.init(tid, a.D, [&](int r) { return row_at(r, 0, a.gs); });
   auto copy = [&](int t, unsigned dst) {
-    constexpr int total = RT * TL::kPieces;
-#pragma unroll
-    for (int it = 0; it < (total + 255) / 256; ++it) {
-      if (total % 256 != 0 && it * 256 + wave * 64 >= total) break;
-      const int p = it * 256 + tid, r = p / TL::kPieces;
-      const int ch = (p % TL::kPieces) ^ TL::twist(r);
-      const int row = t * RT + r, token = row / a.G, g = row - token * a.G;
-      const bool ok = row < a.rows && ch * TL::kPer < a.D;
-      const T* qp = Q + (int64_t)token * a.qs[1] + g * a.qs[2] + ch * TL::kPer;
-      const T* gp = GO + (int64_t)token * a.gs[1] + g * a.gs[2] + ch * TL::kPer;
-      copy16(ok ? (const void*)qp : (const void*)g_zero, dst + (it * 256 + wave * 64) * 16);
-      copy16(ok ? (const void*)gp : (const void*)g_zero,
-             dst + C::kTileBytes + (it * 256 + wave * 64) * 16);
+    const int token0 = t * RT / a.G;
+    const uint64_t qp = Q + (uint64_t)token0 * a.qs[1] * sizeof(T), gp = GO + (uint64_t)token0 * a.gs[1] * sizeof(T);
+    if (regular && (t + 1) * RT <= a.rows) {
+      sq.copy(qp, dst, wave0);
+      sg.copy(gp, dst + C::kTileBytes, wave0);
+    } else {  // rows past the end read the tile's first: their weights are 0
+      auto at = [&](const int64_t* st) {
+        return [=, &a](int it, unsigned o) {
+          const int r = Stage<T, DP, RT, 256>::row_of(it, tid), row = t * RT + r;
+          return o - row_at(r, 0, st) + row_at(row < a.rows ? row : t * RT, token0, st);
+        };
+      };
+      sq.copy(qp, dst, wave0, at(a.qs));
+      sg.copy(gp, dst + C::kTileBytes, wave0, at(a.gs));
     }
     // RT logarithms, then RT deltas (the rows are padded to whole tiles there)
-    if (wave == 0) {
-      const float* src = RT == 64 ? lse + t * RT + lane
-                                  : (half ? delta : lse) + t * RT + (lane & 31);
-      copy4(src, dst + 2 * C::kTileBytes);
-    }
-    if (RT == 64 && wave == 1) copy4(delta + t * RT + lane, dst + 2 * C::kTileBytes + 256);
+    const uint64_t lp = reinterpret_cast<uint64_t>(lse + t * RT), dp = reinterpret_cast<uint64_t>(delta + t * RT);
+    if (wave == 0 && lane < RT) copy4(lp, lane * 4, dst + 2 * C::kTileBytes);
+    if (wave == 1 && lane < RT) copy4(dp, lane * 4, dst + 2 * C::kTileBytes + RT * 4);
   };
 
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -301,23 +299,25 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
 
-  if (tb < te) copy(tb, lds);
-  for (int t = tb, buf = 0; t < te; ++t, buf ^= 1) {
+  int t = tb;
+  if (t < te) copy(t, lds);
+  auto step = [&](auto buf) {
+    constexpr int kAt = decltype(buf)::value * C::kBuf;
     publish();
-    const unsigned qt = lds + buf * C::kBuf, gt = qt + C::kTileBytes, st = gt + C::kTileBytes;
-    if (t + 1 < te) copy(t + 1, lds + (buf ^ 1) * C::kBuf);
-    if (j0 >= keys) continue;
+    if (t + 1 < te) copy(t + 1, lds + (C::kBuf - kAt));
+    const unsigned st = lds + kAt + 2 * C::kTileBytes;
+    if (j0 >= keys) return;
     bool edge = false;
     if (a.band > 0) {
       const int64_t r0 = (int64_t)t * RT, r1 = r0 + RT - 1;
       const int64_t first = (int64_t)j0 * a.G, last = ((int64_t)j0 + 31 + a.band) * a.G - 1;
-      if (r1 < first || r0 > last) continue;
+      if (r1 < first || r0 > last) return;
       edge = r0 < (int64_t)(j0 + 31) * a.G || r1 >= ((int64_t)j0 + a.band) * a.G;
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      f32x16 p = mma_rows<T, DP>(qt, 32 * rb, k, lane);
-      f32x16 ds = mma_rows<T, DP>(gt, 32 * rb, v, lane);
+      f32x16 p = mma_rows<T, DP>(from, kAt, 32 * rb, k);
+      f32x16 ds = mma_rows<T, DP>(from, kAt + C::kTileBytes, 32 * rb, v);
       if (edge) {
         const int64_t first = (int64_t)j * a.G, width = (int64_t)a.band * a.G;
         const int64_t off = (int64_t)t * RT + 32 * rb + 4 * half - first;
@@ -346,9 +346,15 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
           ds[r] = x;
         }
       }
-      mma_transposed<T, DP>(dv, gt, 32 * rb, p, lane);
-      mma_transposed<T, DP>(dk, qt, 32 * rb, ds, lane);
+      mma_transposed<T, DP>(dv, from, kAt + C::kTileBytes, 32 * rb, p);
+      mma_transposed<T, DP>(dk, from, kAt, 32 * rb, ds);
     }
+  };
+  while (t < te) {
+    step(std::integral_constant<int, 0>{});
+    if (++t >= te) break;
+    step(std::integral_constant<int, 1>{});
+    ++t;
   }
   if (j >= a.Lk) return;
   const int64_t out = (((int64_t)b * a.Lk + j) * a.KV + kv) * a.D;

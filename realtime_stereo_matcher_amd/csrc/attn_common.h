@@ -90,26 +90,26 @@ template <typename V>
 __device__ __forceinline__ void lds_put(unsigned addr, V v) {
   *reinterpret_cast<__attribute__((address_space(3))) V*>(addr) = v;
 }
-// 16 (4) bytes a lane from global memory into LDS at a wave's base + 16 (4) * lane, without a
-// register in between.  Inline, because the compiler would wait for every such copy in flight
-// before each LDS read; the kernels wait themselves (wait_copies) before the barrier that
-// publishes a tile.
-__device__ __forceinline__ void copy16(const void* src, unsigned dst) {
+// 16 (4) bytes a lane, from a uniform base and a lane's offset, into LDS at a wave's base + 16 (4) *
+// lane, without a register in between.  Inline, because the compiler would wait for every such copy
+// in flight before each LDS read; the kernels wait themselves (wait_copies, publish) before a tile is
+// read.
+__device__ __forceinline__ void copy16(uint64_t base, unsigned off, unsigned dst) {
   unsigned keep;
   asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(keep)
-      : "v"(src), "s"(dst)
+      : "s"(base), "v"(off), "s"(dst)
       : "memory");
 }
-__device__ __forceinline__ void copy4(const void* src, unsigned dst) {
+__device__ __forceinline__ void copy4(uint64_t base, unsigned off, unsigned dst) {
   unsigned keep;
   asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\t"
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %2, %1\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(keep)
-      : "v"(src), "s"(dst)
+      : "s"(base), "v"(off), "s"(dst)
       : "memory");
 }
 __device__ __forceinline__ void wait_copies() {
@@ -119,77 +119,138 @@ __device__ __forceinline__ void publish() {  // this wave's copies done, then ev
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// what rows past the end, masked keys and columns past the head's width read instead
-static __device__ const unsigned g_zero[4] = {0, 0, 0, 0};
-
-// A tile of rows x DP values, in 16-byte pieces.  Piece `ch` of row `row` sits at ch ^ twist(row):
-// the 8 rows that a 16-byte read serves at once, and the 4 rows x 32 bytes of a transposing read,
-// then fall on different banks (rows are 64 to 512 bytes apart, a multiple of the bank count).
+// A tile of rows x DP values in LDS, in 16-byte pieces.  Piece `ch` of row `row` sits at
+// ch ^ twist(row).  LDS serves 256 bytes a cycle: 16 lanes of a 16-byte read (16 rows, the same
+// piece) or 32 lanes of a transposing read (4 rows, 64 bytes each), and the twist puts both on
+// different banks whatever the rows' length (64 to 512 bytes).
 template <typename T, int DP> struct Tile {
   static constexpr int kPer = 16 / (int)sizeof(T);
   static constexpr int kPieces = DP / kPer;  // of a row
   static constexpr int kRowBytes = DP * (int)sizeof(T);
   static constexpr int kSteps = sizeof(T) == 4 ? DP / 8 : DP / 16;  // row-operand reads
   static __device__ __forceinline__ int twist(int row) {
-    if constexpr (sizeof(T) == 4) return row & 7;
-    if constexpr (kPieces >= 8) return ((row & 3) << 1) | ((row >> 2) & 1);
-    return (row & 2) | ((row >> 2) & 1);
-  }
-  // ROWS rows from `base` (row stride `stride`), row `row0` first, by NT threads (`tid`); `ok(row)`
-  // says which rows of the tile exist.  A wave without a whole instruction left does nothing.
-  template <int ROWS, int NT, typename OK>
-  static __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, unsigned dst,
-                                              int tid, int D, OK ok) {
-    constexpr int total = ROWS * kPieces;
-    static_assert(total % 64 == 0, "whole wave instructions");
-    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
-#pragma unroll
-    for (int it = 0; it < (total + NT - 1) / NT; ++it) {
-      if (total % NT != 0 && it * NT + wave0 >= total) break;
-      const int p = it * NT + tid;
-      const int row = p / kPieces;
-      const int ch = (p % kPieces) ^ twist(row);
-      const T* src = base + (int64_t)(row0 + row) * stride + ch * kPer;
-      const bool there = ok(it, row) && ch * kPer < D;
-      copy16(there ? (const void*)src : (const void*)g_zero, dst + (it * NT + wave0) * 16);
-    }
-  }
-  // left operand with the tile's rows as its rows: row `row`, step s
-  static __device__ __forceinline__ Frag<T> row_op(unsigned tile, int row, int s,
-                                                                 int half) {
-    const int ch = (2 * s + half) ^ twist(row);
-    return lds_get<Frag<T>>(tile + row * kRowBytes + ch * 16);
+    if constexpr (kRowBytes == 64) return (row >> 2) & 3;
+    if constexpr (kRowBytes == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    if constexpr (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+    return (((row >> 2) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1);
   }
 };
 
-// registers of a block that hold 4 (fp32) or 8 (16-bit) consecutive contraction steps
-__device__ __forceinline__ int crow(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+// The copies of a tile of ROWS rows by NT threads: a lane's offset in each instruction, from the
+// tile's first row.  Pieces past the head's width read its first piece: finite values that meet
+// zeros in the other operand, or columns that are not stored.
+template <typename T, int DP, int ROWS, int NT> struct Stage {
+  using TL = Tile<T, DP>;
+  static constexpr int kTotal = ROWS * TL::kPieces, kN = (kTotal + NT - 1) / NT;
+  static_assert(kTotal % 64 == 0, "whole wave instructions");
+  unsigned off[kN];
+  static __device__ __forceinline__ int row_of(int it, int tid) { return (it * NT + tid) / TL::kPieces; }
+  template <typename F> __device__ __forceinline__ void init(int tid, int D, F row_offset) {
+#pragma unroll
+    for (int it = 0; it < kN; ++it) {
+      const int row = row_of(it, tid), ch = ((it * NT + tid) % TL::kPieces) ^ TL::twist(row);
+      off[it] = row_offset(row) + (ch * TL::kPer < D ? ch * 16 : 0);
+    }
+  }
+  // `adjust(it, offset)`: the offset to read instead
+  template <typename F>
+  __device__ __forceinline__ void copy(uint64_t base, unsigned dst, int wave0, F adjust) const {
+#pragma unroll
+    for (int it = 0; it < kN; ++it) {
+      if (kTotal % NT != 0 && it * NT + wave0 >= kTotal) break;
+      copy16(base, adjust(it, off[it]), dst + (it * NT + wave0) * 16);
+    }
+  }
+  __device__ __forceinline__ void copy(uint64_t base, unsigned dst, int wave0) const {
+    copy(base, dst, wave0, [](int, unsigned o) { return o; });
+  }
+  // Rows whose bit is clear (past the end, masked) read the tile's first row whose bit is set: the
+  // scores they give are replaced by -inf, and their values are finite if that row's are.
+  __device__ __forceinline__ void copy(uint64_t base, unsigned dst, int wave0, int tid, uint64_t bits,
+                                       unsigned row_bytes) const {
+    const int first = __builtin_ctzll(bits);
+    copy(base, dst, wave0, [&](int it, unsigned o) {
+      const int row = row_of(it, tid);
+      return (bits >> row) & 1 ? o : o + (unsigned)((first - row) * (int)row_bytes);
+    });
+  }
+};
+
+// A wave's reads of tiles whose LDS addresses differ by constants: the lane's part of every address
+// (a twist is an exclusive or, so each piece has its own) is formed once.
+template <typename T, int DP> struct Reads {
+  using TL = Tile<T, DP>;
+  static constexpr bool kWide = sizeof(T) == 4;
+  unsigned row[kWide ? 1 : TL::kSteps], col[kWide ? 1 : DP / 32][2];
+  int lane;
+  __device__ __forceinline__ Reads(unsigned lds, int lane_) : lane(lane_) {
+    const int half = lane >> 5;
+    if constexpr (kWide) {
+      row[0] = lds;
+    } else {
+      const int r = lane & 31;
+#pragma unroll
+      for (int c = 0; c < TL::kSteps; ++c)
+        row[c] = lds + r * TL::kRowBytes + ((2 * c + half) ^ TL::twist(r)) * 16;
+      // ds_read_tr16_b64: in each 16 lanes, lane i receives column i of the 4 x 16 values whose row
+      // j the lanes 4j .. 4j+3 address
+      const int g = (lane >> 4) & 1, l16 = lane & 15;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int q = 8 * u + 4 * half + (l16 >> 2);
+          col[db][u] = lds + q * TL::kRowBytes +
+                       ((4 * db + 2 * g + ((l16 & 3) >> 1)) ^ TL::twist(q)) * 16 + (l16 & 1) * 8;
+        }
+    }
+  }
+  // left operand with the tile's rows as its rows: rows row0 .. row0+31 (row0 a multiple of 32), step c
+  __device__ __forceinline__ Frag<T> rows(int tile, int row0, int c) const {
+    if constexpr (kWide) {
+      const int r = lane & 31, ch = (2 * c + (lane >> 5)) ^ TL::twist(r);
+      return lds_get<Frag<T>>(row[0] + tile + (row0 + r) * TL::kRowBytes + ch * 16);
+    } else {
+      return lds_get<Frag<T>>(row[c] + (tile + row0 * TL::kRowBytes));
+    }
+  }
+  // the same transposed, 16-bit: rows row0 + 16 s .. + 15 as the contraction of column block db
+  __device__ __forceinline__ Frag<T> columns(int tile, int row0, int s, int db) const {
+    static_assert(!kWide, "16-bit types");
+    typedef __attribute__((address_space(3))) s16x4 lds_s4;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const unsigned at = tile + (row0 + 16 * s) * TL::kRowBytes;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[db][0] + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[db][1] + at));
+    const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(Frag<T>, both);
+  }
+  // fp32: row `row0 + crow(r)` of the tile, a lane's column of block db
+  __device__ __forceinline__ float column(int tile, int row0, int r, int db) const {
+    static_assert(kWide, "fp32");
+    const int c = lane & 31, q = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+    const int ch = (8 * db + (c >> 2)) ^ TL::twist(q);
+    return lds_get<float>(row[0] + tile + q * TL::kRowBytes + ch * 16 + (c & 3) * 4);
+  }
+};
 
 // acc[n][db] += (tile rows row0 .. row0+31, transposed) * block[n], where a block holds a 32x32
 // result (tile rows x lane columns): values of the tile's column are the rows of the product.  N
 // products share the reads of the tile.
 template <typename T, int DP, int N>
-__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[N][DP / 32], unsigned tile, int row0,
-                                               const f32x16 (&block)[N], int lane) {
-  using TL = Tile<T, DP>;
+__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[N][DP / 32], const Reads<T, DP>& from,
+                                               int tile, int row0, const f32x16 (&block)[N]) {
   if constexpr (sizeof(T) == 4) {
-    const int half = lane >> 5, col = lane & 31;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = row0 + crow(r, half);
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) {
-        const int ch = (8 * db + (col >> 2)) ^ TL::twist(row);
-        const float a = lds_get<float>(tile + row * TL::kRowBytes + ch * 16 + (col & 3) * 4);
+        const float a = from.column(tile, row0, r, db);
 #pragma unroll
         for (int n = 0; n < N; ++n)
           acc[n][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, block[n][r], acc[n][db], 0, 0, 0);
       }
-    }
   } else {
-    // ds_read_tr16_b64: in each 16 lanes, lane i receives column i of the 4 x 16 values whose
-    // row j the lanes 4j .. 4j+3 address
-    const int half = lane >> 5, g = (lane >> 4) & 1, l16 = lane & 15;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       Frag<T> p[N];
@@ -199,38 +260,26 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[N][DP / 32], unsign
         for (int e = 0; e < 8; ++e) Mma<T>::put(p[n], e, block[n][8 * s + e]);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) {
-        s16x4 lo, hi;
-        const int row = 4 * half + (l16 >> 2);
-        const int ch = (4 * db + 2 * g + ((l16 & 3) >> 1)) ^ TL::twist(row);
-        const unsigned at = tile + (row0 + 16 * s + row) * TL::kRowBytes + ch * 16 + (l16 & 1) * 8;
-        typedef __attribute__((address_space(3))) s16x4 lds_s4;
-        lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(at));
-        hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_s4*>(at + 8 * TL::kRowBytes));
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const Frag<T> a = from.columns(tile, row0, s, db);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-          acc[n][db] = Mma<T>::mma(__builtin_bit_cast(Frag<T>, both), p[n], acc[n][db]);
+        for (int n = 0; n < N; ++n) acc[n][db] = Mma<T>::mma(a, p[n], acc[n][db]);
       }
     }
   }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], const Reads<T, DP>& from, int tile,
+                                               int row0, const f32x16& block) {
+  mma_transposed<T, DP, 1>(reinterpret_cast<f32x16(&)[1][DP / 32]>(acc), from, tile, row0,
+                           reinterpret_cast<const f32x16(&)[1]>(block));
 }
 
 // a row in registers, as the right operand of all steps over its values
 template <typename T, int DP> using RowOps = Frag<T>[Tile<T, DP>::kSteps];
 
-template <typename T, int DP>
-__device__ __forceinline__ void mma_transposed(f32x16 (&acc)[DP / 32], unsigned tile, int row0,
-                                               const f32x16& block, int lane) {
-  mma_transposed<T, DP, 1>(reinterpret_cast<f32x16(&)[1][DP / 32]>(acc), tile, row0,
-                           reinterpret_cast<const f32x16(&)[1]>(block), lane);
-}
-
 // right operand of one row (a query or a key) a lane, straight from global memory
 template <typename T, int DP>
-__device__ __forceinline__ void load_rows(RowOps<T, DP>& f, const T* row, bool there,
-                                          int half, int D) {
+__device__ __forceinline__ void load_rows(RowOps<T, DP>& f, const T* row, bool there, int half, int D) {
   using TL = Tile<T, DP>;
 #pragma unroll
   for (int s = 0; s < TL::kSteps; ++s) {
@@ -243,16 +292,57 @@ __device__ __forceinline__ void load_rows(RowOps<T, DP>& f, const T* row, bool t
 
 // the tile's rows row0 .. row0+31 times the lanes' columns
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 mma_rows(unsigned tile, int row0,
-                                           const RowOps<T, DP>& f, int lane) {
+__device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, int row0,
+                                           const RowOps<T, DP>& f) {
   f32x16 s;
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-  for (int c = 0; c < Tile<T, DP>::kSteps; ++c)
-    s = Mma<T>::mma(Tile<T, DP>::row_op(tile, row0 + (lane & 31), c, lane >> 5), f[c], s);
+  for (int c = 0; c < Tile<T, DP>::kSteps; ++c) s = Mma<T>::mma(from.rows(tile, row0, c), f[c], s);
   return s;
 }
+
+// the keys that lie outside the length or the mask of a 32-key block: -inf.  Bit j of `w`: key j
+// counts; a lane holds keys 8 (r/4) + 4 half + r%4.
+__device__ __forceinline__ void mask_block(f32x16& s, unsigned w, int half) {
+  w >>= 4 * half;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+}
+// and those outside the band of the lane's token, `ahead` = token - the block's first key
+__device__ __forceinline__ void band_block(f32x16& s, int ahead, int band, int half) {
+  ahead -= 4 * half;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    s[r] = (unsigned)(ahead - (8 * (r >> 2) + (r & 3))) < (unsigned)band ? s[r] : -INFINITY;
+}
+
+// The key tiles of a row tile: which there are, and which keys of each count.
+template <int KT, bool KMASK> struct Keys {
+  static constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
+  const uint8_t* mask;
+  int keys, tb, te;
+  __device__ __forceinline__ Keys(const Args& a, int b, int first_row, int tile_rows)
+      : mask(KMASK ? a.mask + (int64_t)b * a.Lk : nullptr),
+        keys(a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk) {
+    int lo = 0, hi = keys;
+    if (a.band > 0) {  // the tiles inside the band of some row
+      const int last = min(first_row + tile_rows, a.rows) - 1;
+      lo = max(0, first_row / a.G - a.band + 1);
+      hi = min(keys, last / a.G + 1);
+    }
+    tb = lo / KT;
+    te = hi > lo ? (hi + KT - 1) / KT : tb;
+  }
+  __device__ __forceinline__ int byte(int t, int lane) const {
+    const int j = t * KT + lane;
+    return lane < KT && t < te && j < keys ? mask[j] : 0;
+  }
+  __device__ __forceinline__ uint64_t by_length(int t) const {
+    const int n = keys - t * KT;
+    return n >= KT ? kAll : n <= 0 ? 0ull : (1ull << n) - 1;
+  }
+};
 
 // both halves of the wave see both halves' values
 __device__ __forceinline__ float other_half_max(float v) {
@@ -299,16 +389,14 @@ __device__ __forceinline__ unsigned xcd_id() {
   return x * per + min(x, more) + (blockIdx.x >> 3);
 }
 
-__device__ __forceinline__ int key_count(const Args& a, int b) {
-  return a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
-}
-
 int64_t fwd_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV, int64_t D);
 int64_t bwd_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV);
 int check_problem(const char* what, int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
                   int64_t KV, int64_t D, float scale, int64_t band);
+// `group` > 0: tiles of 64 rows, `group` heads side by side, are copied by 32-bit offsets from their
+// first token
 int read_strides3(const int64_t* s, int64_t L, int64_t H, int64_t D, int dtype, const void* base,
-                  int64_t* out, const char* name);
+                  int64_t* out, int group, const char* name);
 int fwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st);
 int bwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st);
 

@@ -7,6 +7,7 @@
 // (they are divided by l, formed against the same m, at the end; weights up to 2^8 lose nothing in
 // any of the types).
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 
@@ -15,29 +16,38 @@ namespace attn {
 
 namespace {
 
-// FEW: at most 32 query rows (single tokens with shared heads): the waves hold the same rows and
-// take the key tiles in turn, each with its own LDS, and join at the end.
-template <typename T, int DP, bool FEW> struct Cfg {
+// How the waves of a workgroup share the work:
+//   FEW       at most 32 query rows (single tokens with shared heads): all waves hold the same rows and
+//             take the key tiles in turn, each with its own LDS and without barriers
+//   GROUPS    1: four waves, 32 rows each; 2: eight waves, 32 rows for each pair, which takes the even
+//             and the odd key tiles
+// Waves that hold the same rows join their sums and statistics through LDS at the end.
+template <typename T, int DP, bool FEW, int GROUPS> struct Cfg {
   static constexpr int kTile = sizeof(T) == 4 ? 32 : (FEW && DP == 128) ? 32 : 64;  // keys
-  static constexpr int kWaves = FEW && sizeof(T) == 4 && DP == 128 ? 2 : 4;
+  static constexpr int kWaves = FEW ? (sizeof(T) == 4 && DP == 128 ? 2 : 4) : 4 * GROUPS;
   static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kParts = FEW ? kWaves : GROUPS;  // of the keys
   static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
   static constexpr int kBufBytes = 2 * kTileBytes;  // keys and values
-  static constexpr int kLds = 2 * kBufBytes * (FEW ? kWaves : 1);
+  // two buffers a part; the join needs a wave's sums and statistics each
+  static constexpr int kTiles = 2 * kBufBytes * kParts;
+  static constexpr int kJoin = kParts > 1 ? kWaves * (32 * (DP + 4) * 4 + 256) : 0;
+  static constexpr int kLds = kTiles > kJoin ? kTiles : kJoin;
 };
 
 constexpr float kLazy = 8.f;
 
-template <typename T, int DP, bool KMASK, bool FEW>
-__global__ __launch_bounds__((Cfg<T, DP, FEW>::kThreads), (FEW || sizeof(T) == 4 ? 1 : 2))
+template <typename T, int DP, bool KMASK, bool FEW, int GROUPS>
+__global__ __launch_bounds__((Cfg<T, DP, FEW, GROUPS>::kThreads), (FEW || (sizeof(T) == 4 && DP == 128) ? 1 : 2))
 void attn_fwd(Args a) {
-  using C = Cfg<T, DP, FEW>;
-  using TL = Tile<T, DP>;
-  using frag = Frag<T>;
-  constexpr int KT = C::kTile, KB = KT / 32;
+  using C = Cfg<T, DP, FEW, GROUPS>;
+  constexpr int KT = C::kTile, KB = KT / 32, kTileRows = FEW ? kFew : kRows;
+  constexpr int kCopiers = FEW ? 64 : 256;  // threads that fetch a tile
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = FEW ? wave : wave >> 2;  // of the keys
+  const int ctid = FEW ? lane : tid & 255, cwave0 = FEW ? 0 : (wave & 3) * 64;
 
   unsigned id = xcd_id();
   const int rt = id % a.row_tiles;
@@ -46,56 +56,39 @@ void attn_fwd(Args a) {
   id /= a.splits;
   const int kv = id % a.KV, b = id / a.KV;
 
-  const int wg_row0 = rt * (FEW ? kFew : kRows);
-  const int row0 = wg_row0 + (FEW ? 0 : 32 * wave);  // of this wave
-  const int row = row0 + (lane & 31);                // of this lane
+  const int wg_row0 = rt * kTileRows;
+  const int row0 = wg_row0 + (FEW ? 0 : 32 * (wave & 3));  // of this wave
+  const int row = row0 + (lane & 31);                      // of this lane
   const int token = row / a.G, head = kv * a.G + row % a.G;
   const bool there = row < a.rows;
 
-  // key tiles of the workgroup: up to the sequence's length, inside the band of its rows, and of
-  // those this split's share
-  const int keys = key_count(a, b);
-  int jlo = 0, jhi = keys;
-  if (a.band > 0) {
-    const int last = min(wg_row0 + (FEW ? kFew : kRows), a.rows) - 1;
-    jlo = max(0, wg_row0 / a.G - a.band + 1);
-    jhi = min(keys, last / a.G + 1);
-  }
-  int tb = jlo / KT, te = jhi > jlo ? (jhi + KT - 1) / KT : tb;
+  Keys<KT, KMASK> keys(a, b, wg_row0, kTileRows);
   if (a.splits > 1) {
-    const int per = (te - tb + a.splits - 1) / a.splits;
-    tb += split * per;
-    te = min(te, tb + per);
+    const int per = (keys.te - keys.tb + a.splits - 1) / a.splits;
+    keys.tb += split * per;
+    keys.te = min(keys.te, keys.tb + per);
   }
 
-  const T* K = static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2];
-  const T* V = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
-  frag q[TL::kSteps];
+  RowOps<T, DP> q;
   load_rows<T, DP>(q, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)token * a.qs[1] +
                           head * a.qs[2], there, half, a.D);
 
-  const unsigned lds = lds_addr(smem) + (FEW ? wave * 2 * C::kBufBytes : 0);
-  const uint8_t* mask = KMASK ? a.mask + (int64_t)b * a.Lk : nullptr;
-  const int step = FEW ? C::kWaves : 1;
-
-  // bit j: key j of the tile exists and is not masked
-  auto mask_byte = [&](int t) -> int {
-    const int j = t * KT + lane;
-    return lane < KT && t < te && j < keys ? mask[j] : 0;
-  };
-  auto length_bits = [&](int t) -> uint64_t {
-    const int n = keys - t * KT;
-    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
-  };
-  constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
+  const unsigned lds = lds_addr(smem) + part * 2 * C::kBufBytes;
+  const Reads<T, DP> from(lds, lane);
+  const unsigned kb_row = (unsigned)a.ks[1] * sizeof(T), vb_row = (unsigned)a.vs[1] * sizeof(T);
+  Stage<T, DP, KT, kCopiers> sk, sv;
+  sk.init(ctid, a.D, [&](int r) { return r * kb_row; });
+  sv.init(ctid, a.D, [&](int r) { return r * vb_row; });
+  const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
+  const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
-    auto ok = [&](int, int r) { return ((bits >> r) & 1) != 0; };
-    if (FEW) {
-      TL::template load<KT, 64>(K, a.ks[1], t * KT, dst, lane, a.D, ok);
-      TL::template load<KT, 64>(V, a.vs[1], t * KT, dst + C::kTileBytes, lane, a.D, ok);
-    } else {
-      TL::template load<KT, C::kThreads>(K, a.ks[1], t * KT, dst, tid, a.D, ok);
-      TL::template load<KT, C::kThreads>(V, a.vs[1], t * KT, dst + C::kTileBytes, tid, a.D, ok);
+    const uint64_t kp = K + (uint64_t)t * KT * kb_row, vp = V + (uint64_t)t * KT * vb_row;
+    if (bits == keys.kAll) {
+      sk.copy(kp, dst, cwave0);
+      sv.copy(vp, dst + C::kTileBytes, cwave0);
+    } else if (bits != 0) {
+      sk.copy(kp, dst, cwave0, ctid, bits, kb_row);
+      sv.copy(vp, dst + C::kTileBytes, cwave0, ctid, bits, vb_row);
     }
   };
 
@@ -106,56 +99,45 @@ void attn_fwd(Args a) {
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  int t = tb + (FEW ? wave : 0);
+  constexpr int kStep = C::kParts;
+  int t = keys.tb + part;
   uint64_t bits = 0;
   int byte = 0;
-  if (t < te) {
-    bits = KMASK ? __ballot(mask_byte(t)) : length_bits(t);
-    if (KMASK) byte = mask_byte(t + step);
+  if (t < keys.te) {
+    bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
     copy(t, lds, bits);
   }
-  for (int buf = 0; t < te; t += step, buf ^= 1) {
+  if (KMASK) byte = keys.byte(t + kStep, lane);
+
+  auto step = [&](auto buf) {
+    constexpr int kBuf = decltype(buf)::value * C::kBufBytes;
     // this tile is in LDS, and nobody reads the other buffer any more
     if (FEW) wait_copies(); else publish();
     uint64_t next = 0;
-    if (t + step < te) {
-      next = KMASK ? __ballot(byte) : length_bits(t + step);
-      if (KMASK) byte = mask_byte(t + 2 * step);
-      copy(t + step, lds + (buf ^ 1) * C::kBufBytes, next);
+    if (t + kStep < keys.te) {
+      next = KMASK ? __ballot(byte) : keys.by_length(t + kStep);
+      if (KMASK) byte = keys.byte(t + 2 * kStep, lane);
+      copy(t + kStep, lds + (C::kBufBytes - kBuf), next);
     }
-    const unsigned kt = lds + buf * C::kBufBytes, vt = kt + C::kTileBytes;
-    const uint64_t seen = bits & kAll;
+    const uint64_t seen = bits;
     bits = next;
+    if (seen == 0) return;  // (also a group's turn past the last tile)
     bool edge = false;
     if (a.band > 0) {
       const int j0 = t * KT, j1 = j0 + KT - 1;
       const int i0 = row0 / a.G, i1 = min(row0 + 31, a.rows - 1) / a.G;
-      if (j0 > i1 || j1 <= i0 - a.band) continue;  // outside this wave's band
+      if (j0 > i1 || j1 <= i0 - a.band) return;  // outside this wave's band
       edge = j1 > i0 || j0 <= i1 - a.band;
     }
-    if (seen == 0) continue;
-
     f32x16 s[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = mma_rows<T, DP>(kt, 32 * kb, q, lane);
-    if (seen != kAll) {
+    for (int kb = 0; kb < KB; ++kb) s[kb] = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
+    if (seen != keys.kAll)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const unsigned w = (unsigned)(seen >> (32 * kb)) >> (4 * half);
+      for (int kb = 0; kb < KB; ++kb) mask_block(s[kb], (unsigned)(seen >> (32 * kb)), half);
+    if (edge)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[kb][r] = (w >> (8 * (r >> 2) + (r & 3))) & 1 ? s[kb][r] : -INFINITY;
-      }
-    }
-    if (edge) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int d = token - (t * KT + 32 * kb + 4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[kb][r] = (unsigned)(d - (8 * (r >> 2) + (r & 3))) < (unsigned)a.band ? s[kb][r] : -INFINITY;
-      }
-    }
+      for (int kb = 0; kb < KB; ++kb) band_block(s[kb], token - (t * KT + 32 * kb), a.band, half);
     float mx = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -173,25 +155,37 @@ void attn_fwd(Args a) {
       m = mn;
     }
     const float mc = m == -INFINITY ? 0.f : m * a.c;
+    float part_l[2] = {0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.c, -mc));
-        l += s[kb][r];
+        part_l[r & 1] += s[kb][r];
       }
+    l += part_l[0] + part_l[1];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) mma_transposed<T, DP>(o, vt, 32 * kb, s[kb], lane);
+    for (int kb = 0; kb < KB; ++kb) mma_transposed<T, DP>(o, from, kBuf + C::kTileBytes, 32 * kb, s[kb]);
+  };
+  // every wave passes the same number of barriers: the groups' first tiles decide
+  const int end = FEW ? keys.te : keys.te + part;
+  while (t < end) {
+    step(std::integral_constant<int, 0>{});
+    t += kStep;
+    if (t >= end) break;
+    step(std::integral_constant<int, 1>{});
+    t += kStep;
   }
   l = other_half_sum(l);
 
-  const int64_t at = ((int64_t)b * a.KV + kv) * a.rows + row;  // of this lane's row
-  if constexpr (FEW) {
-    // join the waves: rows x DP partial sums and the statistics of each wave
+  if constexpr (C::kParts > 1) {
+    // join the waves that hold the same rows: rows x DP partial sums and statistics of each wave
     constexpr int kPitch = (DP + 4) * 4, kWaveBytes = 32 * kPitch + 256;
-    static_assert(C::kWaves * kWaveBytes <= C::kLds, "the join fits the tiles' LDS");
+    constexpr int kSets = FEW ? 1 : 4;  // of rows
+    static_assert(C::kWaves * kWaveBytes == C::kJoin, "the join's LDS");
+    const unsigned base = lds_addr(smem);
     __syncthreads();
-    const unsigned mine = lds_addr(smem) + wave * kWaveBytes;
+    const unsigned mine = base + wave * kWaveBytes;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -203,31 +197,32 @@ void attn_fwd(Args a) {
       lds_put(mine + 32 * kPitch + 128 + lane * 4, l);
     }
     __syncthreads();
-    for (int p = tid; p < 32 * (DP / 4); p += C::kThreads) {
-      const int r = p / (DP / 4), d = 4 * (p % (DP / 4)), grow = wg_row0 + r;
+    for (int p = tid; p < kTileRows * (DP / 4); p += C::kThreads) {
+      const int tr = p / (DP / 4), r = tr & 31, d = 4 * (p % (DP / 4)), grow = wg_row0 + tr;
       if (grow >= a.rows || d >= a.D) continue;
-      float top = -INFINITY, mw[C::kWaves];
+      const unsigned set = base + (tr >> 5) * kWaveBytes;
+      float top = -INFINITY, mw[C::kParts];
 #pragma unroll
-      for (int w = 0; w < C::kWaves; ++w) {
-        mw[w] = lds_get<float>(lds_addr(smem) + w * kWaveBytes + 32 * kPitch + r * 4);
+      for (int w = 0; w < C::kParts; ++w) {
+        mw[w] = lds_get<float>(set + w * kSets * kWaveBytes + 32 * kPitch + r * 4);
         top = fmaxf(top, mw[w]);
       }
-      const float base = top == -INFINITY ? 0.f : top;
+      const float from_m = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < C::kWaves; ++w) {
-        const unsigned from = lds_addr(smem) + w * kWaveBytes;
-        const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw[w] - base) * a.c);
-        sum = fmaf(f, lds_get<float>(from + 32 * kPitch + 128 + r * 4), sum);
-        const f32x4 x = lds_get<f32x4>(from + r * kPitch + d * 4);
+      for (int w = 0; w < C::kParts; ++w) {
+        const unsigned at = set + w * kSets * kWaveBytes;
+        const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw[w] - from_m) * a.c);
+        sum = fmaf(f, lds_get<float>(at + 32 * kPitch + 128 + r * 4), sum);
+        const f32x4 x = lds_get<f32x4>(at + r * kPitch + d * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(f, x[e], v[e]);
       }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= inv;
-      const float lse = sum == 0.f ? -INFINITY : fmaf(base, a.c, __builtin_amdgcn_logf(sum)) * kLn2;
+      const float lse = sum == 0.f ? -INFINITY : fmaf(from_m, a.c, __builtin_amdgcn_logf(sum)) * kLn2;
       const int64_t ra = ((int64_t)b * a.KV + kv) * a.rows + grow;
       if (a.splits > 1) {
         const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + ra;
@@ -241,6 +236,7 @@ void attn_fwd(Args a) {
     }
   } else {
     if (!there) return;
+    const int64_t at = ((int64_t)b * a.KV + kv) * a.rows + row;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float lse = l == 0.f ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l)) * kLn2;
     if (a.splits > 1) {
@@ -286,15 +282,15 @@ __global__ __launch_bounds__(256) void attn_join(Args a) {
   if (d == 0 && a.lse) a.lse[r] = sum == 0.f ? -INFINITY : base + __builtin_amdgcn_logf(sum) * kLn2;
 }
 
-template <typename T, int DP, bool KMASK, bool FEW>
+template <typename T, int DP, bool KMASK, bool FEW, int GROUPS>
 int launch(const Args& a, hipStream_t st) {
-  using C = Cfg<T, DP, FEW>;
+  using C = Cfg<T, DP, FEW, GROUPS>;
   static std::atomic<unsigned long long> done{0};
-  const void* kern = reinterpret_cast<const void*>(&attn_fwd<T, DP, KMASK, FEW>);
+  const void* kern = reinterpret_cast<const void*>(&attn_fwd<T, DP, KMASK, FEW, GROUPS>);
   if (const int rc = ensure_lds_limit(kern, C::kLds, stream_device(st), done)) return rc;
   const int64_t grid = (int64_t)a.B * a.KV * a.splits * a.row_tiles;
   if (grid > 0x7fffffffll) return fail(SM_EINVAL, "cross_attention: too many row tiles");
-  attn_fwd<T, DP, KMASK, FEW><<<dim3((unsigned)grid), C::kThreads, C::kLds, st>>>(a);
+  attn_fwd<T, DP, KMASK, FEW, GROUPS><<<dim3((unsigned)grid), C::kThreads, C::kLds, st>>>(a);
   if (const int rc = check_launch("cross_attention")) return rc;
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.B * a.KV * a.rows * (a.D / 4);
@@ -304,16 +300,24 @@ int launch(const Args& a, hipStream_t st) {
   return SM_OK;
 }
 
+template <typename T, int DP, bool KMASK>
+int by_rows(const Args& a, hipStream_t st) {
+  if (a.rows <= kFew) return launch<T, DP, KMASK, true, 1>(a, st);
+  // a launch that leaves a compute unit one workgroup gives it eight waves instead of four (wide fp32
+  // rows need the registers of four)
+  if constexpr (sizeof(T) == 2 || DP < 128) {
+    const int64_t wgs = (int64_t)a.B * a.KV * a.splits * a.row_tiles;
+    if (wgs <= kCus) return launch<T, DP, KMASK, false, 2>(a, st);
+  }
+  return launch<T, DP, KMASK, false, 1>(a, st);
+}
+
 template <typename T>
 int by_width(const Args& a, hipStream_t st) {
-  const bool few = a.rows <= kFew, km = a.mask != nullptr;
-#define SM_ATTN_WIDTH(DP)                                                            \
-  return few ? (km ? launch<T, DP, true, true>(a, st) : launch<T, DP, false, true>(a, st)) \
-             : (km ? launch<T, DP, true, false>(a, st) : launch<T, DP, false, false>(a, st));
-  if (a.D <= 32) { SM_ATTN_WIDTH(32) }
-  if (a.D <= 64) { SM_ATTN_WIDTH(64) }
-  SM_ATTN_WIDTH(128)
-#undef SM_ATTN_WIDTH
+  const bool km = a.mask != nullptr;
+  if (a.D <= 32) return km ? by_rows<T, 32, true>(a, st) : by_rows<T, 32, false>(a, st);
+  if (a.D <= 64) return km ? by_rows<T, 64, true>(a, st) : by_rows<T, 64, false>(a, st);
+  return km ? by_rows<T, 128, true>(a, st) : by_rows<T, 128, false>(a, st);
 }
 
 // How many workgroups share the keys of one row tile: as many as fill the card's 256 compute units
@@ -346,7 +350,7 @@ int check_problem(const char* what, int dtype, int64_t B, int64_t Lq, int64_t Lk
 }
 
 int read_strides3(const int64_t* s, int64_t L, int64_t H, int64_t D, int dtype, const void* base,
-                  int64_t* out, const char* name) {
+                  int64_t* out, int group, const char* name) {
   if (s == nullptr) {
     out[0] = L * H * D;
     out[1] = H * D;
@@ -359,6 +363,12 @@ int read_strides3(const int64_t* s, int64_t L, int64_t H, int64_t D, int dtype, 
     if (out[i] < 0) return fail(SM_EINVAL, std::string(name) + ": negative strides are not supported");
     if (out[i] % per != 0)
       return fail(SM_EINVAL, std::string(name) + ": strides must be multiples of 16 bytes");
+  }
+  if (group > 0) {
+    const int64_t most = (1ll << 31) / elem_size(dtype);
+    const bool far = out[1] >= most / 128 || (group > 1 && out[2] >= most / 2 / group) ||
+                     (64 / group + 2) * out[1] + (group - 1) * out[2] >= most;
+    if (far) return fail(SM_EINVAL, std::string(name) + ": tokens or heads too far apart");
   }
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0)
     return fail(SM_EINVAL, std::string(name) + ": must be 16-byte aligned");

@@ -611,13 +611,15 @@ def _tensors(what, **named):
             raise TypeError(f"{what}: {name} must be a tensor")
 
 
-def _token_ready(t):
+def _token_ready(t, group=1):
     """(tensor, its (batch, token, head) strides): unit stride of the values, the others and the
-    address multiples of 16 bytes -- a copy where they are not."""
+    address multiples of 16 bytes, 64 rows of ``group`` heads within 2^31 bytes -- a copy where they
+    are not."""
     per = 16 // t.element_size()
     st = tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()))
     if ((t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0
-            and st[0] % per == 0 and st[1] % per == 0 and st[2] % per == 0):
+            and st[0] % per == 0 and st[1] % per == 0 and st[2] % per == 0
+            and st[1] < (1 << 24) // t.element_size() and (group == 1 or st[2] * group < (1 << 27))):
         return t, st
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride()[:3]
@@ -661,10 +663,10 @@ def _attention_backward(q, k, v, out, lse, dout, lengths, mask, scale, band):
         dv = torch.empty_like(dk)
         if dq.numel() or dk.numel():
             lib = _lib.load()
-            q, qs = _token_ready(q)
+            q, qs = _token_ready(q, h // kv)
             k, ks = _token_ready(k)
             v, vs = _token_ready(v)
-            dout, gs = _token_ready(dout)
+            dout, gs = _token_ready(dout, h // kv)
             nws = lib.sm_cross_attention_backward_workspace_bytes(b, lq, h, kv)
             ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
             _lib.check(lib.sm_cross_attention_backward(

@@ -198,13 +198,13 @@ def _abi(fn, *args):
 def test_abi_refuses():
     """The C entries return an error before any launch (the pointers are never read)."""
     P = 1 << 20  # a pointer that is 16-byte aligned
-    ok = dict(dtype=_lib.SM_BF16, B=1, Lq=4, Lk=8, H=4, KV=2, D=16, scale=0.25, band=0, out=P, q=P, st=None,
+    ok = dict(dtype=_lib.SM_BF16, B=1, Lq=4, Lk=8, H=4, KV=2, D=16, scale=0.25, band=0, out=P, q=P, st=None, kst=None,
               ws=None, nws=0)
 
     def fwd(**kw):
         a = {**ok, **kw}
         return _abi("sm_cross_attention", a["q"], P, P, a["out"], None, a["dtype"], a["B"], a["Lq"], a["Lk"],
-                    a["H"], a["KV"], a["D"], a["st"], None, None, a["scale"], a["band"], None, None, a["ws"],
+                    a["H"], a["KV"], a["D"], a["st"], a["kst"], None, a["scale"], a["band"], None, None, a["ws"],
                     a["nws"], None)
 
     I3 = ctypes.c_int64 * 3
@@ -219,6 +219,7 @@ def test_abi_refuses():
             (dict(out=None), _lib.SM_EINVAL, "output"), (dict(out=P + 8), _lib.SM_EINVAL, "output"),
             (dict(q=P + 2), _lib.SM_EINVAL, "aligned"), (dict(q=None), _lib.SM_EINVAL, "null"),
             (dict(st=I3(256, 64, 12)), _lib.SM_EINVAL, "strides"), (dict(st=I3(-64, 64, 16)), _lib.SM_EINVAL, "negative"),
+            (dict(kst=I3(0, 1 << 23, 16)), _lib.SM_EINVAL, "far apart"),
             (dict(nws=-1), _lib.SM_EINVAL, "workspace"),
             (dict(Lq=1, Lk=8192), _lib.SM_EINVAL, "workspace")]:
         rc, msg = fwd(**kw)
@@ -446,8 +447,8 @@ def test_cross_attention_small_fp16_gradients():
 @gpu
 @pytest.mark.parametrize("lq", [1, 40])
 def test_cross_attention_far_offsets(lq):
-    """Tokens 2^26 values apart: the last key lies past 2^32 bytes and 2^31 values."""
-    apart, lk, d = 1 << 26, 40, 64
+    """Keys 2^23 - 2^16 values apart: the last one lies past 2^32 bytes and 2^31 values."""
+    apart, lk, d = (1 << 23) - (1 << 16), 300, 64
     store = torch.empty(lk * apart, dtype=torch.bfloat16, device="cuda")
     gen = torch.Generator().manual_seed(6)
     q, k, v = (normal(gen, 1, n, 1, d, dtype=torch.bfloat16) for n in (lq, lk, lk))
