@@ -46,11 +46,17 @@ _ALGOS = {"auto": _lib.SM_IP_AUTO, "valu": _lib.SM_IP_VALU, "mfma": _lib.SM_IP_M
 
 
 # ----------------------------------------------------------------------------------- plumbing
+_tracing = None  # library.tracing, once imported (library.py imports this module)
+
+
 def _traced():
     """Under torch.jit.trace or a compiler the call is routed through torch.ops.stereocv, so the
     traced graph holds the operator instead of its output as a constant (library.py)."""
-    from . import library
-    return library.tracing()
+    global _tracing
+    if _tracing is None:
+        from . import library
+        _tracing = library.tracing
+    return _tracing()
 
 
 def _ops():
@@ -142,6 +148,12 @@ def _run(fn, *inputs):
 
 def _ptr(t):
     return t.data_ptr()
+
+
+# the current stream's handle by device index: torch's own raw accessor where it has one, since
+# building a Stream object costs more than the smallest kernels' launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 _HALF = (torch.float16, torch.bfloat16)
@@ -605,83 +617,91 @@ def _token_dtype(t, what, name):
     return code
 
 
-def _tensors(what, **named):
-    for name, t in named.items():
+def _tensors(what, *named):
+    for name, t in zip(named[::2], named[1::2]):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} must be a tensor")
+
+
+def _on_device(fn):
+    """Run ``fn(dev, ...)`` with ``dev`` the current device (where its launches go)."""
+    def run(dev, *args):
+        if torch.cuda.current_device() == dev.index:
+            return fn(dev, *args)
+        with torch.cuda.device(dev):
+            return fn(dev, *args)
+    return run
 
 
 def _token_ready(t, group=1):
     """(tensor, its (batch, token, head) strides): unit stride of the values, the others and the
     address multiples of 16 bytes, 64 rows of ``group`` heads within 2^31 bytes -- a copy where they
     are not."""
+    if group == 1 and t.data_ptr() % 16 == 0 and t.is_contiguous():
+        return t, None
     per = 16 // t.element_size()
     st = tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()))
     if ((t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0
             and st[0] % per == 0 and st[1] % per == 0 and st[2] % per == 0
             and st[1] < (1 << 24) // t.element_size() and (group == 1 or st[2] * group < (1 << 27))):
-        return t, st
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()[:3]
+        return t, _lib.int64s(*st)
+    return t.clone(memory_format=torch.contiguous_format), None
 
 
 def _grads_wanted(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-def _attention_forward(q, k, v, lengths, mask, scale, band, want_lse):
+@_on_device
+def _attention_forward(dev, q, k, v, lengths, mask, scale, band, want_lse):
     b, lq, h, d = q.shape
     lk, kv = k.shape[1], k.shape[2]
-    dev = q.device
-    with torch.cuda.device(dev):
-        out = torch.empty((b, lq, h, d), dtype=q.dtype, device=dev)
-        lse = torch.empty((b, kv, lq * (h // kv)) if kv else (b, 0, 0), dtype=torch.float32,
-                          device=dev) if want_lse else None
-        if out.numel():
-            lib = _lib.load()
-            q, qs = _token_ready(q)
-            k, ks = _token_ready(k)
-            v, vs = _token_ready(v)
-            nws = lib.sm_cross_attention_workspace_bytes(b, lq, lk, h, kv, d)
-            ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-            _lib.check(lib.sm_cross_attention(
-                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse) if want_lse else None,
-                _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, _lib.int64s(*qs), _lib.int64s(*ks),
-                _lib.int64s(*vs), scale, band, None if lengths is None else _ptr(lengths),
-                None if mask is None else _ptr(mask), None if ws is None else _ptr(ws), nws,
-                _stream(dev)), "sm_cross_attention")
+    out = q.new_empty((b, lq, h, d))
+    lse = q.new_empty((b, kv, lq * (h // kv)) if kv else (b, 0, 0), dtype=torch.float32) if want_lse else None
+    if out.numel():
+        lib = _lib.load()
+        q, qs = _token_ready(q)
+        k, ks = _token_ready(k)
+        v, vs = _token_ready(v)
+        nws = lib.sm_cross_attention_workspace_bytes(b, lq, lk, h, kv, d)
+        ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
+        _lib.check(lib.sm_cross_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
+            _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, qs, ks, vs, scale, band,
+            None if lengths is None else lengths.data_ptr(), None if mask is None else mask.data_ptr(),
+            ws.data_ptr() if nws else None, nws, _raw_stream(dev.index)), "sm_cross_attention")
     return out, lse
 
 
-def _attention_backward(q, k, v, out, lse, dout, lengths, mask, scale, band):
+@_on_device
+def _attention_backward(dev, q, k, v, out, lse, dout, lengths, mask, scale, band):
     b, lq, h, d = q.shape
     lk, kv = k.shape[1], k.shape[2]
-    dev = q.device
-    with torch.cuda.device(dev):
-        dq = torch.empty((b, lq, h, d), dtype=q.dtype, device=dev)
-        dk = torch.empty((b, lk, kv, d), dtype=q.dtype, device=dev)
-        dv = torch.empty_like(dk)
-        if dq.numel() or dk.numel():
-            lib = _lib.load()
-            q, qs = _token_ready(q, h // kv)
-            k, ks = _token_ready(k)
-            v, vs = _token_ready(v)
-            dout, gs = _token_ready(dout, h // kv)
-            nws = lib.sm_cross_attention_backward_workspace_bytes(b, lq, h, kv)
-            ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-            _lib.check(lib.sm_cross_attention_backward(
-                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk),
-                _ptr(dv), _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, _lib.int64s(*qs),
-                _lib.int64s(*ks), _lib.int64s(*vs), _lib.int64s(*gs), scale, band,
-                None if lengths is None else _ptr(lengths), None if mask is None else _ptr(mask),
-                None if ws is None else _ptr(ws), nws, _stream(dev)), "sm_cross_attention_backward")
+    dq = q.new_empty((b, lq, h, d))
+    dk = q.new_empty((b, lk, kv, d))
+    dv = q.new_empty((b, lk, kv, d))
+    if dq.numel() or dk.numel():
+        lib = _lib.load()
+        group = h // kv if kv else 1
+        q, qs = _token_ready(q, group)
+        k, ks = _token_ready(k)
+        v, vs = _token_ready(v)
+        dout, gs = _token_ready(dout, group)
+        nws = lib.sm_cross_attention_backward_workspace_bytes(b, lq, h, kv)
+        ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
+        _lib.check(lib.sm_cross_attention_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, qs, ks,
+            vs, gs, scale, band, None if lengths is None else lengths.data_ptr(),
+            None if mask is None else mask.data_ptr(), ws.data_ptr() if nws else None, nws,
+            _raw_stream(dev.index)), "sm_cross_attention_backward")
     return dq, dk, dv
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale, band):
-        out, lse = _attention_forward(q, k, v, lengths, mask, scale, band, True)
+        out, lse = _attention_forward(q.device, q, k, v, lengths, mask, scale, band, True)
         ctx.save_for_backward(q, k, v, out, lse, lengths, mask)
         ctx.scale, ctx.band = scale, band
         ctx.mark_non_differentiable(lse)
@@ -691,13 +711,13 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, _):
         q, k, v, out, lse, lengths, mask = ctx.saved_tensors
-        return (*_attention_backward(q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
+        return (*_attention_backward(q.device, q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
                 None, None, None, None)
 
 
 def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_mask):
     what = "cross_attention"
-    _tensors(what, query=query, key=key, value=value)
+    _tensors(what, "query", query, "key", key, "value", value)
     if query.dim() != 4 or key.dim() != 4:
         raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(query.shape)} and "
                            f"{tuple(key.shape)}")
@@ -724,12 +744,12 @@ def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_
         if not 1 <= band < 1 << 30:
             raise ValueError(f"{what}: max_disparity must be positive, got {band}")
     if key_lengths is not None:
-        _tensors(what, key_lengths=key_lengths)
+        _tensors(what, "key_lengths", key_lengths)
         if key_lengths.shape != (b,) or key_lengths.dtype not in (torch.int32, torch.int64):
             raise RuntimeError(f"{what}: key_lengths must be {b} int32 or int64 values, got "
                                f"{tuple(key_lengths.shape)} {key_lengths.dtype}")
     if key_mask is not None:
-        _tensors(what, key_mask=key_mask)
+        _tensors(what, "key_mask", key_mask)
         if key_mask.shape != (b, lk) or key_mask.dtype != torch.bool:
             raise RuntimeError(f"{what}: key_mask must be ({b}, {lk}) truth values, got "
                                f"{tuple(key_mask.shape)} {key_mask.dtype}")
@@ -775,7 +795,7 @@ def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengt
         if _grads_wanted(query, key, value):
             out, lse = _CrossAttention.apply(query, key, value, lengths, mask, scale, band)
         else:
-            out, lse = _attention_forward(query, key, value, lengths, mask, scale, band, return_lse)
+            out, lse = _attention_forward(query.device, query, key, value, lengths, mask, scale, band, return_lse)
     if not return_lse:
         return out
     b, lq, h, _ = query.shape
@@ -820,23 +840,25 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_len
     return f.to(device) if device is not None else f
 
 
-def _rotary_run(x, positions, frequencies, interleaved, amplitude, inverse):
+@_on_device
+def _rotary_run(dev, x, positions, frequencies, interleaved, amplitude, inverse):
     b, l, h, d = x.shape
-    dev = x.device
-    with torch.cuda.device(dev):
-        y = torch.empty((b, l, h, d), dtype=x.dtype, device=dev)
-        if y.numel():
+    y = x.new_empty((b, l, h, d))
+    if y.numel():
+        st = None
+        if not x.is_contiguous():
             if x.stride(3) != 1 and d > 1:
                 x = x.contiguous()
-            flags = ((_lib.SM_ROTARY_INTERLEAVED if interleaved else 0)
-                     | (_lib.SM_ROTARY_INVERSE if inverse else 0)
-                     | (_lib.SM_ROTARY_POS64 if positions.dtype == torch.int64 else 0))
-            st = (0 if n == 1 else s for n, s in zip(x.shape[:3], x.stride()))
-            ps = positions.stride(0) if positions.dim() == 2 and b > 1 else 0
-            _lib.check(_lib.load().sm_rotary(
-                _ptr(x), _ptr(positions), _ptr(frequencies), _ptr(y), _TOKEN_DTYPES[x.dtype], b, l, h,
-                d, 2 * frequencies.numel(), _lib.int64s(*st), ps, flags, amplitude, _stream(dev)),
-                "sm_rotary")
+            else:
+                st = _lib.int64s(*(0 if n == 1 else s for n, s in zip(x.shape[:3], x.stride())))
+        flags = ((_lib.SM_ROTARY_INTERLEAVED if interleaved else 0)
+                 | (_lib.SM_ROTARY_INVERSE if inverse else 0)
+                 | (_lib.SM_ROTARY_POS64 if positions.dtype == torch.int64 else 0))
+        ps = positions.stride(0) if positions.dim() == 2 and b > 1 else 0
+        _lib.check(_lib.load().sm_rotary(
+            x.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), y.data_ptr(), _TOKEN_DTYPES[x.dtype],
+            b, l, h, d, 2 * frequencies.numel(), st, ps, flags, amplitude, _raw_stream(dev.index)),
+            "sm_rotary")
     return y
 
 
@@ -845,12 +867,12 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, frequencies, interleaved, amplitude):
         ctx.save_for_backward(positions, frequencies)
         ctx.how = interleaved, amplitude
-        return _rotary_run(x, positions, frequencies, interleaved, amplitude, False)
+        return _rotary_run(x.device, x, positions, frequencies, interleaved, amplitude, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return (_rotary_run(dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
+        return (_rotary_run(dy.device, dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
 
 
 def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
@@ -866,7 +888,7 @@ def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
     if _traced():
         return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
     what = "rotary"
-    _tensors(what, x=x, positions=positions, frequencies=frequencies)
+    _tensors(what, "x", x, "positions", positions, "frequencies", frequencies)
     if x.dim() != 4:
         raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(x.shape)}")
     _token_dtype(x, what, "x")
@@ -890,12 +912,14 @@ def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
     how = layout == "interleaved", float(amplitude)
     if _grads_wanted(x):
         return _Rotary.apply(x, positions, frequencies, *how)
-    return _rotary_run(x, positions, frequencies, *how, False)
+    return _rotary_run(x.device, x, positions, frequencies, *how, False)
 
 
 # ------------------------------------------------------------------------------------- RMS norm
 def _rows(t, c):
     """(the tensor as rows of c contiguous values, their stride)."""
+    if t.is_contiguous():
+        return t, c
     t = t.reshape(-1, c)
     if c > 1 and t.stride(1) != 1:
         t = t.contiguous()
@@ -903,7 +927,9 @@ def _rows(t, c):
 
 
 def _norm_checks(what, x, weight, residual, eps):
-    _tensors(what, x=x, weight=weight, **({} if residual is None else {"residual": residual}))
+    _tensors(what, "x", x, "weight", weight)
+    if residual is not None:
+        _tensors(what, "residual", residual)
     if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
         raise RuntimeError(f"{what}: expected (..., C) rows and (C,) weight, got {tuple(x.shape)} and "
                            f"{tuple(weight.shape)}")
@@ -917,62 +943,64 @@ def _norm_checks(what, x, weight, residual, eps):
         raise RuntimeError(f"{what}: x/residual shape mismatch {tuple(x.shape)} vs {tuple(residual.shape)}")
     if not 0.0 <= float(eps) < 3.4e38:
         raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
-    _device_check(x, weight, *(() if residual is None else (residual,)))
+    if residual is None:
+        _device_check(x, weight)
+    else:
+        _device_check(x, weight, residual)
 
 
-def _norm_forward(x, weight, residual, eps, e4m3=None):
+@_on_device
+def _norm_forward(dev, x, weight, residual, eps, e4m3=None):
     """(y, summed or None), or with ``e4m3`` (the group) (q, scales, summed or None)."""
-    dev, c = x.device, x.shape[-1]
+    c = x.shape[-1]
     shape, code = x.shape, _TOKEN_DTYPES[x.dtype]
-    with torch.cuda.device(dev):
-        summed = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
-        y = torch.empty(shape, dtype=x.dtype if e4m3 is None else torch.float8_e4m3fn, device=dev)
-        scales = None
-        if e4m3 is not None:
-            per = -(-c // e4m3) if e4m3 else 1
-            scales = torch.empty((*shape[:-1], per), dtype=torch.float32, device=dev)
-        if y.numel():
-            x, xs = _rows(x, c)
-            rcode, rs, rp, sp = code, c, None, None
-            if residual is not None:
-                residual, rs = _rows(residual, c)
-                rcode, rp, sp = _TOKEN_DTYPES[residual.dtype], _ptr(residual), _ptr(summed)
-            weight = weight.contiguous()
-            wcode = _TOKEN_DTYPES[weight.dtype]
-            lib = _lib.load()
-            if e4m3 is None:
-                _lib.check(lib.sm_rms_norm(_ptr(x), rp, _ptr(weight), _ptr(y), sp, code, rcode, wcode,
-                                           x.shape[0], c, xs, rs, eps, _stream(dev)), "sm_rms_norm")
-            else:
-                _lib.check(lib.sm_rms_norm_e4m3(
-                    _ptr(x), rp, _ptr(weight), _ptr(y), _ptr(scales), sp, code, rcode, wcode, x.shape[0],
-                    c, xs, rs, e4m3, eps, _stream(dev)), "sm_rms_norm_e4m3")
+    summed = None if residual is None else residual.new_empty(shape)
+    y = x.new_empty(shape, dtype=x.dtype if e4m3 is None else torch.float8_e4m3fn)
+    scales = None
+    if e4m3 is not None:
+        scales = x.new_empty((*shape[:-1], -(-c // e4m3) if e4m3 else 1), dtype=torch.float32)
+    if y.numel():
+        x, xs = _rows(x, c)
+        rcode, rs, rp, sp = code, c, None, None
+        if residual is not None:
+            residual, rs = _rows(residual, c)
+            rcode, rp, sp = _TOKEN_DTYPES[residual.dtype], residual.data_ptr(), summed.data_ptr()
+        weight = weight.contiguous()
+        wcode, n, st = _TOKEN_DTYPES[weight.dtype], y.numel() // c, _raw_stream(dev.index)
+        lib = _lib.load()
+        if e4m3 is None:
+            _lib.check(lib.sm_rms_norm(x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), sp, code, rcode,
+                                       wcode, n, c, xs, rs, eps, st), "sm_rms_norm")
+        else:
+            _lib.check(lib.sm_rms_norm_e4m3(
+                x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), scales.data_ptr(), sp, code, rcode, wcode,
+                n, c, xs, rs, e4m3, eps, st), "sm_rms_norm_e4m3")
     return (y, summed) if e4m3 is None else (y, scales, summed)
 
 
-def _norm_backward(summed, weight, dy, dsummed, dtype, eps):
+@_on_device
+def _norm_backward(dev, summed, weight, dy, dsummed, dtype, eps):
     """(dx, dresidual in summed's type or None where that is dx, dweight)."""
-    dev, c = summed.device, summed.shape[-1]
-    with torch.cuda.device(dev):
-        dx = torch.empty(summed.shape, dtype=dtype, device=dev)
-        dres = None if summed.dtype == dtype else torch.empty_like(dx, dtype=summed.dtype)
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
-        n = summed.numel() // c
-        lib = _lib.load()
-        nws = lib.sm_rms_norm_backward_workspace_bytes(n, c)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-        summed, ss = _rows(summed, c)
-        dy, ys = _rows(dy, c)
-        zs, zp = c, None
-        if dsummed is not None:
-            dsummed, zs = _rows(dsummed, c)
-            zp = _ptr(dsummed)
-        weight = weight.contiguous()
-        _lib.check(lib.sm_rms_norm_backward(
-            _ptr(summed), _ptr(weight), _ptr(dy), zp, _ptr(dx), None if dres is None else _ptr(dres),
-            _ptr(dw), _TOKEN_DTYPES[dtype], _TOKEN_DTYPES[summed.dtype], _TOKEN_DTYPES[weight.dtype], n,
-            c, ss, ys, zs, eps, None if ws is None else _ptr(ws), nws, _stream(dev)),
-            "sm_rms_norm_backward")
+    c = summed.shape[-1]
+    dx = summed.new_empty(summed.shape, dtype=dtype)
+    dres = None if summed.dtype == dtype else summed.new_empty(summed.shape)
+    dw = weight.new_empty(weight.shape)
+    n = summed.numel() // c
+    lib = _lib.load()
+    nws = lib.sm_rms_norm_backward_workspace_bytes(n, c)
+    ws = summed.new_empty(nws, dtype=torch.uint8) if nws else None
+    summed, ss = _rows(summed, c)
+    dy, ys = _rows(dy, c)
+    zs, zp = c, None
+    if dsummed is not None:
+        dsummed, zs = _rows(dsummed, c)
+        zp = dsummed.data_ptr()
+    weight = weight.contiguous()
+    _lib.check(lib.sm_rms_norm_backward(
+        summed.data_ptr(), weight.data_ptr(), dy.data_ptr(), zp, dx.data_ptr(),
+        None if dres is None else dres.data_ptr(), dw.data_ptr(), _TOKEN_DTYPES[dtype],
+        _TOKEN_DTYPES[summed.dtype], _TOKEN_DTYPES[weight.dtype], n, c, ss, ys, zs, eps,
+        ws.data_ptr() if nws else None, nws, _raw_stream(dev.index)), "sm_rms_norm_backward")
     return dx, dres, dw
 
 
@@ -981,20 +1009,20 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, eps):
         ctx.save_for_backward(x, weight)
         ctx.eps = eps
-        return _norm_forward(x, weight, None, eps)[0]
+        return _norm_forward(x.device, x, weight, None, eps)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
-        dx, _, dw = _norm_backward(x, weight, dy, None, x.dtype, ctx.eps)
+        dx, _, dw = _norm_backward(x.device, x, weight, dy, None, x.dtype, ctx.eps)
         return dx, dw, None
 
 
 class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        y, summed = _norm_forward(x, weight, residual, eps)
+        y, summed = _norm_forward(x.device, x, weight, residual, eps)
         ctx.save_for_backward(summed, weight)
         ctx.eps, ctx.dtype = eps, x.dtype
         ctx.set_materialize_grads(False)
@@ -1008,7 +1036,7 @@ class _AddRmsNorm(torch.autograd.Function):
             if dsummed is None:
                 return None, None, None, None
             return dsummed.to(ctx.dtype), None, dsummed, None
-        dx, dres, dw = _norm_backward(summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
+        dx, dres, dw = _norm_backward(summed.device, summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
         return dx, dw, dx if dres is None else dres, None
 
 
@@ -1030,10 +1058,10 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     if residual is None:
         if _grads_wanted(x, weight):
             return _RmsNorm.apply(x, weight, eps)
-        return _norm_forward(x, weight, None, eps)[0]
+        return _norm_forward(x.device, x, weight, None, eps)[0]
     if _grads_wanted(x, weight, residual):
         return _AddRmsNorm.apply(x, weight, residual, eps)
-    return _norm_forward(x, weight, residual, eps)
+    return _norm_forward(x.device, x, weight, residual, eps)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
@@ -1053,5 +1081,5 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
     _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
     if _grads_wanted(x, weight, residual):
         raise NotImplementedError("rms_norm_e4m3 is forward only: call it under torch.no_grad()")
-    out = _norm_forward(x, weight, residual, float(eps), group or 0)
+    out = _norm_forward(x.device, x, weight, residual, float(eps), group or 0)
     return out[:2] if residual is None else out

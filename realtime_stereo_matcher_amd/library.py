@@ -268,7 +268,7 @@ def _attn(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
           max_disparity: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor]:
     scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
                                                      key_lengths, key_mask)
-    return F._attention_forward(query, key, value, lengths, mask, scale, band, True)
+    return F._attention_forward(query.device, query, key, value, lengths, mask, scale, band, True)
 
 
 def _attn_fake(query, key, value, key_lengths=None, key_mask=None, scale=None, max_disparity=None):
@@ -307,7 +307,7 @@ def _attn_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     if tuple(lse.shape) != (query.shape[0], kv, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise RuntimeError("cross_attention_backward: lse must be the forward call's")
     F._device_check(query, out, lse, dout)
-    return F._attention_backward(query, key, value, out, lse, dout, lengths, mask, scale, band)
+    return F._attention_backward(query.device, query, key, value, out, lse, dout, lengths, mask, scale, band)
 
 
 def _attn_backward_fake(query, key, value, out, lse, dout, key_lengths=None, key_mask=None, scale=None,
@@ -320,7 +320,7 @@ def _rot(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, la
     with _Inside(), torch.no_grad():
         if not inverse:
             return F.rotary(x, positions, frequencies, layout, amplitude)
-        return F._rotary_run(x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
+        return F._rotary_run(x.device, x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
                              amplitude, True)
 
 
@@ -386,7 +386,7 @@ def _norm_backward(summed: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor,
     F._norm_checks("rms_norm_backward", dy, weight, summed, eps)
     if dsummed is not None and (dsummed.shape != summed.shape or dsummed.dtype != summed.dtype):
         raise RuntimeError("rms_norm_backward: dsummed must have summed's shape and type")
-    dx, dres, dw = F._norm_backward(summed, weight, dy, dsummed, dy.dtype, eps)
+    dx, dres, dw = F._norm_backward(summed.device, summed, weight, dy, dsummed, dy.dtype, eps)
     return dx, dx.new_empty(0, dtype=summed.dtype) if dres is None else dres, dw
 
 
