@@ -387,6 +387,8 @@ int attention_args(attn::Args* a, const char* what, const void* query, const voi
   a->G = KV > 0 ? (int)(H / KV) : 1;
   a->D = (int)D;
   a->rows = a->Lq * a->G;
+  a->by_group = attn::Divide(a->G);
+  a->by_kv = attn::Divide(KV);
   a->band = (int)max_disparity;
   a->splits = 1;
   a->scale = scale;

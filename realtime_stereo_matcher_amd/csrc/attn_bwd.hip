@@ -50,12 +50,10 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  unsigned id = xcd_id();
-  const int rt = id % a.row_tiles;
-  id /= a.row_tiles;
-  const int kv = id % a.KV, b = id / a.KV;
+  const unsigned id = xcd_id(), bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
+  const int rt = id - bkv * a.row_tiles, kv = bkv - b * a.KV;
   const int wg_row0 = rt * kRows, row0 = wg_row0 + 32 * wave, row = row0 + (lane & 31);
-  const int token = row / a.G, head = kv * a.G + row % a.G;
+  const int token = a.by_group(row), head = kv * a.G + row - token * a.G;
   const bool there = row < a.rows;
 
   Keys<KT, KMASK> keys(a, b, wg_row0, kRows);
@@ -164,20 +162,16 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     const uint64_t seen = bits;
     bits = next;
     if (seen == 0) return;
-    bool edge = false;
-    if (a.band > 0) {
-      const int j0 = t * KT, j1 = j0 + KT - 1;
-      const int i0 = row0 / a.G, i1 = min(row0 + 31, a.rows - 1) / a.G;
-      if (j0 > i1 || j1 <= i0 - a.band) return;
-      edge = j1 > i0 || j0 <= i1 - a.band;
-    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
+      const BandOf in(a, row0, t * KT + 32 * kb, 32);
+      const unsigned seen32 = (unsigned)(seen >> (32 * kb));
+      if (!in.some || seen32 == 0) continue;
       f32x16 s = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
       f32x16 ds[N];  // and the weights
       ds[0] = mma_rows<T, DP>(from, kBuf + C::kTileBytes, 32 * kb, g);
-      if (seen != keys.kAll) mask_block(s, (unsigned)(seen >> (32 * kb)), half);
-      if (edge) band_block(s, token - (t * KT + 32 * kb), a.band, half);
+      if (!in.all || seen32 != ~0u)
+        mask_block(s, a.band > 0 ? band_bits(seen32, token - (t * KT + 32 * kb), a.band) : seen32, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));
@@ -219,11 +213,8 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  unsigned id = xcd_id();
-  const int key_tiles = (a.Lk + kRows - 1) / kRows;
-  const int jt = id % key_tiles;
-  id /= key_tiles;
-  const int kv = id % a.KV, b = id / a.KV;
+  const unsigned id = xcd_id(), bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
+  const int jt = id - bkv * a.key_tiles, kv = bkv - b * a.KV;
   const int wg_j0 = jt * kRows, j0 = wg_j0 + 32 * wave, j = j0 + (lane & 31);
   const int keys = a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
   const bool there = j < keys && (!KMASK || a.mask[(int64_t)b * a.Lk + min(j, a.Lk - 1)] != 0);
@@ -263,16 +254,16 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   const uint64_t GO = reinterpret_cast<uint64_t>(static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)kv * a.G * a.gs[2]);
   // Row t RT + r is token (t RT + r) / G: where G divides RT the offsets from the tile's first token
   // are the same in every tile.
-  const bool regular = RT % a.G == 0;
+  const bool regular = (RT & (a.G - 1)) == 0 && (a.G & (a.G - 1)) == 0;
   auto row_at = [&](int row, int token0, const int64_t* st) -> unsigned {
-    const int token = row / a.G, g = row - token * a.G;
+    const int token = a.by_group(row), g = row - token * a.G;
     return ((token - token0) * (unsigned)st[1] + g * (unsigned)st[2]) * (unsigned)sizeof(T);
   };
   Stage<T, DP, RT, 256> sq, sg;
   sq.init(tid, a.D, [&](int r) { return row_at(r, 0, a.qs); });
   sg.init(tid, a.D, [&](int r) { return row_at(r, 0, a.gs); });
   auto copy = [&](int t, unsigned dst) {
-    const int token0 = t * RT / a.G;
+    const int token0 = a.by_group(t * RT);
     const uint64_t qp = Q + (uint64_t)token0 * a.qs[1] * sizeof(T), gp = GO + (uint64_t)token0 * a.gs[1] * sizeof(T);
     if (regular && (t + 1) * RT <= a.rows) {
       sq.copy(qp, dst, wave0);
@@ -307,25 +298,24 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     if (t + 1 < te) copy(t + 1, lds + (C::kBuf - kAt));
     const unsigned st = lds + kAt + 2 * C::kTileBytes;
     if (j0 >= keys) return;
-    bool edge = false;
-    if (a.band > 0) {
-      const int64_t r0 = (int64_t)t * RT, r1 = r0 + RT - 1;
-      const int64_t first = (int64_t)j0 * a.G, last = ((int64_t)j0 + 31 + a.band) * a.G - 1;
-      if (r1 < first || r0 > last) return;
-      edge = r0 < (int64_t)(j0 + 31) * a.G || r1 >= ((int64_t)j0 + a.band) * a.G;
-    }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
+      // row r is inside key j's band iff 0 <= r - j G < band G
+      bool edge = false;
+      if (a.band > 0) {
+        const int64_t r0 = (int64_t)t * RT + 32 * rb, r1 = r0 + 31;
+        const int64_t first = (int64_t)j0 * a.G, last = ((int64_t)j0 + 31 + a.band) * a.G - 1;
+        if (r1 < first || r0 > last) continue;
+        edge = r0 < (int64_t)(j0 + 31) * a.G || r1 >= ((int64_t)j0 + a.band) * a.G;
+      }
       f32x16 p = mma_rows<T, DP>(from, kAt, 32 * rb, k);
       f32x16 ds = mma_rows<T, DP>(from, kAt + C::kTileBytes, 32 * rb, v);
       if (edge) {
-        const int64_t first = (int64_t)j * a.G, width = (int64_t)a.band * a.G;
-        const int64_t off = (int64_t)t * RT + 32 * rb + 4 * half - first;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int64_t x = off + 8 * (r >> 2) + (r & 3);
-          p[r] = x >= 0 && x < width ? p[r] : -INFINITY;
-        }
+        const int64_t first = (int64_t)j * a.G - ((int64_t)t * RT + 32 * rb);  // in the block
+        const int64_t after = first + (int64_t)a.band * a.G;
+        const unsigned upto = after >= 32 ? ~0u : after <= 0 ? 0u : (1u << after) - 1;
+        const unsigned past = first <= 0 ? ~0u : first >= 32 ? 0u : ~0u << first;
+        mask_block(p, upto & past, half);
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -375,7 +365,7 @@ int launch(const Args& a, hipStream_t st) {
   const int dev = stream_device(st);
   if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK>), C::kLdsQ, dev, done_q)) return rc;
   if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dkv<T, DP, KMASK>), C::kLdsKv, dev, done_kv)) return rc;
-  const int64_t bkv = (int64_t)a.B * a.KV, key_tiles = ceil_div(a.Lk, kRows);
+  const int64_t bkv = (int64_t)a.B * a.KV, key_tiles = a.key_tiles;
   if (bkv * a.row_tiles > 0x7fffffffll || bkv * key_tiles > 0x7fffffffll)
     return fail(SM_EINVAL, "cross_attention_backward: too many row tiles");
   if (a.row_tiles > 0) {
@@ -416,6 +406,9 @@ int bwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t
   a.row_lse = static_cast<float*>(workspace);
   a.row_delta = a.row_lse + n * kRows;
   a.tile_max = a.row_delta + n * kRows;
+  a.key_tiles = (int)ceil_div(a.Lk, kRows);
+  a.by_row_tiles = Divide(a.row_tiles);
+  a.by_key_tiles = Divide(a.key_tiles);
   SM_DISPATCH_DTYPE(dtype, T, return by_width<T>(a, st));
   return SM_OK;
 }

@@ -28,6 +28,21 @@ constexpr int kCus = 256;    // compute units of the MI355X: what a launch has t
 constexpr int kRows = 128;   // query rows of a workgroup (32 a wave)
 constexpr int kFew = 32;     // at most so many rows: the waves share the rows and split the keys
 
+// n / d for 0 <= n < 2^31 by a multiplication (division by an invariant integer, Granlund and
+// Montgomery 1994): with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) < 2^32 + 1, n m / 2^(31+l)
+// exceeds n / d by less than 1 / d.
+struct Divide {
+  uint32_t m = 0, shift = 0;
+  Divide() = default;
+  explicit Divide(int64_t d) {
+    d = d < 1 ? 1 : d;
+    while ((int64_t(1) << shift) < d) ++shift;
+    shift += 31;
+    m = (uint32_t)(((uint64_t(1) << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int operator()(unsigned n) const { return (int)(((uint64_t)n * m) >> shift); }
+};
+
 struct Args {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
@@ -41,7 +56,8 @@ struct Args {
   int B, Lq, Lk, H, KV, G, D;
   int rows, row_tiles;    // Lq * G and its tiles: row r is token r / G, head kv * G + r % G
   int band;               // > 0: key j is a candidate of token i iff 0 <= i - j < band
-  int splits;
+  int splits, key_tiles;  // of 128 keys (backward)
+  Divide by_group, by_kv, by_row_tiles, by_splits, by_key_tiles;
   float scale, c;         // c = scale * log2(e): exp(scale x) = exp2(c x)
 };
 
@@ -302,20 +318,37 @@ __device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, i
   return s;
 }
 
-// the keys that lie outside the length or the mask of a 32-key block: -inf.  Bit j of `w`: key j
-// counts; a lane holds keys 8 (r/4) + 4 half + r%4.
-__device__ __forceinline__ void mask_block(f32x16& s, unsigned w, int half) {
-  w >>= 4 * half;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+// The keys of a 32-key block that the lane's token may see, bit j for key j: those that exist and are
+// not masked (`there`, the same for every lane) and, if there is a band, 0 <= ahead - j < band with
+// ahead = token - the block's first key.
+__device__ __forceinline__ unsigned band_bits(unsigned there, int ahead, int band) {
+  const int lo = ahead - band + 1;  // first key inside
+  const unsigned upto = ahead < 0 ? 0u : ahead >= 31 ? ~0u : (2u << ahead) - 1;
+  const unsigned from = lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo;
+  return there & upto & from;
 }
-// and those outside the band of the lane's token, `ahead` = token - the block's first key
-__device__ __forceinline__ void band_block(f32x16& s, int ahead, int band, int half) {
-  ahead -= 4 * half;
+// scores of keys whose bit is clear: -inf.  A lane holds keys 8 (r/4) + 4 half + r%4.  (Two bit
+// operations a score: a compare and a select cost a wait between them.)
+__device__ __forceinline__ void mask_block(f32x16& s, unsigned bits, int half) {
+  const int w = (int)(bits >> (4 * half));
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    s[r] = (unsigned)(ahead - (8 * (r >> 2) + (r & 3))) < (unsigned)band ? s[r] : -INFINITY;
+  for (int r = 0; r < 16; ++r) {
+    const unsigned keep = (unsigned)((w << (31 - (8 * (r >> 2) + (r & 3)))) >> 31);
+    s[r] = __uint_as_float((keep & __float_as_uint(s[r])) | (~keep & 0xff800000u));
+  }
 }
+// whether a block of keys from j0 on touches (`some`), or lies inside (`all`), the band of the 32 rows
+// from row0 on
+struct BandOf {
+  bool some, all;
+  __device__ __forceinline__ BandOf(const Args& a, int row0, int j0, int n) : some(true), all(true) {
+    if (a.band > 0) {
+      const int i0 = a.by_group(row0), i1 = max(i0, a.by_group(min(row0 + 31, a.rows - 1))), j1 = j0 + n - 1;
+      some = j0 <= i1 && j1 > i0 - a.band;
+      all = j1 <= i0 && j0 > i1 - a.band;
+    }
+  }
+};
 
 // The key tiles of a row tile: which there are, and which keys of each count.
 template <int KT, bool KMASK> struct Keys {
@@ -328,8 +361,8 @@ template <int KT, bool KMASK> struct Keys {
     int lo = 0, hi = keys;
     if (a.band > 0) {  // the tiles inside the band of some row
       const int last = min(first_row + tile_rows, a.rows) - 1;
-      lo = max(0, first_row / a.G - a.band + 1);
-      hi = min(keys, last / a.G + 1);
+      lo = max(0, a.by_group(first_row) - a.band + 1);
+      hi = min(keys, a.by_group(last) + 1);
     }
     tb = lo / KT;
     te = hi > lo ? (hi + KT - 1) / KT : tb;

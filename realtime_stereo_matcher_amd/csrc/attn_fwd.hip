@@ -49,17 +49,14 @@ void attn_fwd(Args a) {
   const int part = FEW ? wave : wave >> 2;  // of the keys
   const int ctid = FEW ? lane : tid & 255, cwave0 = FEW ? 0 : (wave & 3) * 64;
 
-  unsigned id = xcd_id();
-  const int rt = id % a.row_tiles;
-  id /= a.row_tiles;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int kv = id % a.KV, b = id / a.KV;
+  const unsigned id = xcd_id();
+  const unsigned by_tile = a.by_row_tiles(id), by_split = a.by_splits(by_tile), b = a.by_kv(by_split);
+  const int rt = id - by_tile * a.row_tiles, split = by_tile - by_split * a.splits, kv = by_split - b * a.KV;
 
   const int wg_row0 = rt * kTileRows;
   const int row0 = wg_row0 + (FEW ? 0 : 32 * (wave & 3));  // of this wave
   const int row = row0 + (lane & 31);                      // of this lane
-  const int token = row / a.G, head = kv * a.G + row % a.G;
+  const int token = a.by_group(row), head = kv * a.G + row - token * a.G;
   const bool there = row < a.rows;
 
   Keys<KT, KMASK> keys(a, b, wg_row0, kTileRows);
@@ -122,22 +119,18 @@ void attn_fwd(Args a) {
     const uint64_t seen = bits;
     bits = next;
     if (seen == 0) return;  // (also a group's turn past the last tile)
-    bool edge = false;
-    if (a.band > 0) {
-      const int j0 = t * KT, j1 = j0 + KT - 1;
-      const int i0 = row0 / a.G, i1 = min(row0 + 31, a.rows - 1) / a.G;
-      if (j0 > i1 || j1 <= i0 - a.band) return;  // outside this wave's band
-      edge = j1 > i0 || j0 <= i1 - a.band;
-    }
+    const BandOf in(a, row0, t * KT, KT);
+    if (!in.some) return;
     f32x16 s[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) s[kb] = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
-    if (seen != keys.kAll)
+    if (!in.all || seen != keys.kAll)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mask_block(s[kb], (unsigned)(seen >> (32 * kb)), half);
-    if (edge)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) band_block(s[kb], token - (t * KT + 32 * kb), a.band, half);
+      for (int kb = 0; kb < KB; ++kb) {
+        unsigned w = (unsigned)(seen >> (32 * kb));
+        if (a.band > 0) w = band_bits(w, token - (t * KT + 32 * kb), a.band);
+        mask_block(s[kb], w, half);
+      }
     float mx = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -229,8 +222,8 @@ void attn_fwd(Args a) {
         *reinterpret_cast<f32x4*>(a.part_o + ps * a.D + d) = v;
         if (d == 0) a.part_l[ps] = lse;
       } else {
-        const int64_t tok = (int64_t)b * a.Lq + grow / a.G;
-        store4<T>(static_cast<T*>(a.out) + (tok * a.H + kv * a.G + grow % a.G) * a.D + d, v);
+        const int i = a.by_group(grow);
+        store4<T>(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + kv * a.G + grow - i * a.G) * a.D + d, v);
         if (d == 0 && a.lse) a.lse[ra] = lse;
       }
     }
@@ -394,6 +387,8 @@ int fwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t
     a.part_o = static_cast<float*>(workspace);
     a.part_l = a.part_o + n * a.D;
   }
+  a.by_row_tiles = Divide(a.row_tiles);
+  a.by_splits = Divide(a.splits);
   SM_DISPATCH_DTYPE(dtype, T, return by_width<T>(a, st));
   return SM_OK;
 }
