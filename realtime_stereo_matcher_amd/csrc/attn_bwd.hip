@@ -26,13 +26,55 @@ namespace smcv {
 namespace attn {
 namespace {
 
-template <typename T, int DP> struct BCfg {
-  static constexpr int kTile = sizeof(T) == 4 || DP == 128 ? 32 : 64;  // streamed rows
+// How the waves of a workgroup share the work, by what the launch has to fill the card with:
+//   kMany  four waves with 32 rows (dkv: keys) each
+//   kSome  eight: two for each 32 rows, which take the even and the odd tiles of the other side
+//   kFew   four (wide fp32: two) for the same 32 rows, which take the tiles in turn, each with its own
+//          LDS and without barriers
+// Waves that hold the same rows add their sums through LDS at the end, in one order.
+enum { kMany = 0, kSome = 1, kFewRows = 2 };
+
+template <typename T, int DP, int MODE> struct BCfg {
+  static constexpr bool kWide = sizeof(T) == 4, kAlone = MODE == kFewRows;
+  static constexpr int kTile = kWide || DP == 128 || kAlone ? 32 : 64;  // streamed rows
+  static constexpr int kSets = kAlone ? 1 : 4;
+  static constexpr int kParts = MODE == kMany ? 1 : MODE == kSome ? 2 : kWide && DP == 128 ? 2 : 4;
+  static constexpr int kWaves = kSets * kParts, kThreads = 64 * kWaves, kTileRows = 32 * kSets;
+  static constexpr int kCopiers = kAlone ? 64 : 256;  // threads that fetch a tile
   static constexpr int kTileBytes = kTile * DP * (int)sizeof(T);
-  static constexpr int kLdsQ = 4 * kTileBytes;               // two buffers of keys and values
-  static constexpr int kBuf = 2 * kTileBytes + 512;           // rows, gradients, lse and delta
-  static constexpr int kLdsKv = 2 * kBuf;
+  static constexpr int kBufQ = 2 * kTileBytes;         // keys and values
+  static constexpr int kBufKv = 2 * kTileBytes + 512;  // rows, gradients, lse and delta
+  static constexpr int kJoin = kParts > 1 ? kWaves * 32 * (DP + 4) * 4 : 0;
+  static constexpr int kLdsQ = kJoin > 2 * kBufQ * kParts ? kJoin : 2 * kBufQ * kParts;
+  static constexpr int kLdsKv = kJoin > 2 * kBufKv * kParts ? kJoin : 2 * kBufKv * kParts;
+  // waves a SIMD: two where the accumulators leave room for them
+  static constexpr int kResident = kAlone || DP == 128 || (kWide && DP == 64) ? 1 : 2;
+  static constexpr bool kHasSome = kWide ? DP <= 32 : DP <= 64;
 };
+
+// out(row of the workgroup, column, 4 values summed over the parts) for the waves' transposed results
+template <typename T, int DP, int SETS, int PARTS, typename F>
+__device__ __forceinline__ void join_columns(unsigned lds, int wave, int lane, int tid,
+                                             const f32x16 (&acc)[DP / 32], F out) {
+  constexpr int kPitch = (DP + 4) * 4, kWave = 32 * kPitch;
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i)
+    lds_put(lds + wave * kWave + (lane & 31) * kPitch + column_at<T, DP>(i, lane >> 5) * 4,
+            column_values<T, DP>(acc, i));
+  __syncthreads();
+  for (int p = tid; p < SETS * 32 * (DP / 4); p += SETS * PARTS * 64) {
+    const int r = p / (DP / 4), d = 4 * (p % (DP / 4));
+    const unsigned at = lds + (r >> 5) * kWave + (r & 31) * kPitch + d * 4;
+    f32x4 v = lds_get<f32x4>(at);
+#pragma unroll
+    for (int w = 1; w < PARTS; ++w) {
+      const f32x4 x = lds_get<f32x4>(at + w * SETS * kWave);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
+    out(r, d, v);
+  }
+}
 
 // the power of two that brings x into [1/2, 1), as an exponent; 0 for 0, infinities and NaN
 __device__ __forceinline__ int down(float x) {
@@ -40,9 +82,10 @@ __device__ __forceinline__ int down(float x) {
   return e == 0 || e == 255 ? 0 : min(126 - e, 100);
 }
 
-template <typename T, int DP, bool KMASK>
-__global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dq(Args a) {
-  using C = BCfg<T, DP>;
+template <typename T, int DP, bool KMASK, int MODE>
+__global__ __launch_bounds__((BCfg<T, DP, MODE>::kThreads), (BCfg<T, DP, MODE>::kResident))
+void attn_dq(Args a) {
+  using C = BCfg<T, DP, MODE>;
   using TL = Tile<T, DP>;
   constexpr int KT = C::kTile, KB = KT / 32;
   constexpr bool kScaled = std::is_same<T, __half>::value;
@@ -52,11 +95,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 
   const unsigned id = xcd_id(), bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
   const int rt = id - bkv * a.row_tiles, kv = bkv - b * a.KV;
-  const int wg_row0 = rt * kRows, row0 = wg_row0 + 32 * wave, row = row0 + (lane & 31);
+  const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
+  const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
+  const int wg_row0 = rt * C::kTileRows, row0 = wg_row0 + 32 * set, row = row0 + (lane & 31);
   const int token = a.by_group(row), head = kv * a.G + row - token * a.G;
   const bool there = row < a.rows;
 
-  Keys<KT, KMASK> keys(a, b, wg_row0, kRows);
+  Keys<KT, KMASK> keys(a, b, wg_row0, C::kTileRows);
 
   const int64_t orow = (((int64_t)b * a.Lq + token) * a.H + head) * a.D;
   RowOps<T, DP> q, g;
@@ -79,12 +124,11 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     delta = other_half_sum(delta);
     most = other_half_max(most);
   }
-  const int64_t n_pad = (int64_t)a.row_tiles * kRows;
-  const int64_t at = ((int64_t)b * a.KV + kv) * n_pad + row;
+  const int64_t at = ((int64_t)b * a.KV + kv) * a.pad_rows + row;
   const float lse = there ? a.lse[((int64_t)b * a.KV + kv) * a.rows + row] : -INFINITY;
   // a row without keys, or past the end: +inf makes every weight that is formed from it 0
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
-  if (half == 0) {
+  if (half == 0 && part == 0) {
     a.row_lse[at] = lse2;
     if constexpr (sizeof(T) == 4) a.row_delta[at] = delta;
   }
@@ -96,10 +140,9 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     if (lane == 0) lds_put(lds_addr(smem) + 4 * wave, top);
     __syncthreads();
     if (tid == 0) {
-      const unsigned at0 = lds_addr(smem);
-      a.tile_max[((int64_t)b * a.KV + kv) * a.row_tiles + rt] =
-          fmaxf(fmaxf(lds_get<float>(at0), lds_get<float>(at0 + 4)),
-                fmaxf(lds_get<float>(at0 + 8), lds_get<float>(at0 + 12)));
+#pragma unroll
+      for (int w = 0; w < C::kSets; ++w) top = fmaxf(top, lds_get<float>(lds_addr(smem) + 4 * w));
+      a.tile_max[((int64_t)b * a.KV + kv) * a.row_tiles + rt] = top;
     }
     __syncthreads();
     shift = down(most);
@@ -111,23 +154,22 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
         Mma<T>::put(g[s], e, __builtin_ldexpf(Mma<T>::get(g[s], e), shift));
   }
 
-  const unsigned lds = lds_addr(smem);
+  const unsigned lds = lds_addr(smem) + part * 2 * C::kBufQ;
   const Reads<T, DP> from(lds, lane);
-  const int wave0 = wave * 64;
   const unsigned kb_row = (unsigned)a.ks[1] * sizeof(T), vb_row = (unsigned)a.vs[1] * sizeof(T);
-  Stage<T, DP, KT, 256> sk, sv;
-  sk.init(tid, a.D, [&](int r) { return r * kb_row; });
-  sv.init(tid, a.D, [&](int r) { return r * vb_row; });
+  Stage<T, DP, KT, C::kCopiers> sk, sv;
+  sk.init(ctid, a.D, [&](int r) { return r * kb_row; });
+  sv.init(ctid, a.D, [&](int r) { return r * vb_row; });
   const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
   const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
     const uint64_t kp = K + (uint64_t)t * KT * kb_row, vp = V + (uint64_t)t * KT * vb_row;
     if (bits == keys.kAll) {
-      sk.copy(kp, dst, wave0);
-      sv.copy(vp, dst + C::kTileBytes, wave0);
+      sk.copy(kp, dst, cwave0);
+      sv.copy(vp, dst + C::kTileBytes, cwave0);
     } else if (bits != 0) {
-      sk.copy(kp, dst, wave0, tid, bits, kb_row);
-      sv.copy(vp, dst + C::kTileBytes, wave0, tid, bits, vb_row);
+      sk.copy(kp, dst, cwave0, ctid, bits, kb_row);
+      sv.copy(vp, dst + C::kTileBytes, cwave0, ctid, bits, vb_row);
     }
   };
 
@@ -142,22 +184,22 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
 
-  int t = keys.tb;
+  int t = keys.tb + part;
   uint64_t bits = 0;
   int byte = 0;
   if (t < keys.te) {
     bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
     copy(t, lds, bits);
   }
-  if (KMASK) byte = keys.byte(t + 1, lane);
-  auto step = [&](auto buf) {
-    constexpr int kBuf = decltype(buf)::value * 2 * C::kTileBytes;
-    publish();
+  if (KMASK) byte = keys.byte(t + C::kParts, lane);
+  auto step = [&](auto buf) __attribute__((always_inline)) {
+    constexpr int kBuf = decltype(buf)::value * C::kBufQ;
+    if (C::kAlone) wait_copies(); else publish();
     uint64_t next = 0;
-    if (t + 1 < keys.te) {
-      next = KMASK ? __ballot(byte) : keys.by_length(t + 1);
-      if (KMASK) byte = keys.byte(t + 2, lane);
-      copy(t + 1, lds + (2 * C::kTileBytes - kBuf), next);
+    if (t + C::kParts < keys.te) {
+      next = KMASK ? __ballot(byte) : keys.by_length(t + C::kParts);
+      if (KMASK) byte = keys.byte(t + 2 * C::kParts, lane);
+      copy(t + C::kParts, lds + (C::kBufQ - kBuf), next);
     }
     const uint64_t seen = bits;
     bits = next;
@@ -184,28 +226,56 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
       mma_transposed<T, DP, N>(dq, from, kBuf, 32 * kb, ds);
     }
   };
-  while (t < keys.te) {
+  // every wave passes the same number of barriers: the parts' first tiles decide
+  const int end = C::kAlone ? keys.te : keys.te + part;
+  while (t < end) {
     step(std::integral_constant<int, 0>{});
-    if (++t >= keys.te) break;
+    t += C::kParts;
+    if (t >= end) break;
     step(std::integral_constant<int, 1>{});
-    ++t;
+    t += C::kParts;
   }
+  const unsigned base = lds_addr(smem);
+  if constexpr (C::kParts > 1) __syncthreads();
   if constexpr (N == 2) {
     sum = other_half_sum(sum);
-    if (half == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift);
+    if constexpr (C::kParts > 1) {
+      if (half == 0) lds_put(base + (wave * 32 + lane) * 4, sum);
+      __syncthreads();
+      sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::kParts; ++w)
+        sum += lds_get<float>(base + ((w * C::kSets + set) * 32 + (lane & 31)) * 4);
+      __syncthreads();
+    }
+    if (half == 0 && part == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift);
     delta -= sum;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(delta, dq[1][db][r], dq[0][db][r]);
   }
-  if (!there) return;
-  store_columns<T, DP>(static_cast<T*>(a.dq) + orow, dq[0], __builtin_ldexpf(a.scale, -shift), half, a.D);
+  const float by = __builtin_ldexpf(a.scale, -shift);
+  if constexpr (C::kParts > 1) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[0][db][r] *= by;
+    join_columns<T, DP, C::kSets, C::kParts>(base, wave, lane, tid, dq[0], [&](int r, int d, f32x4 v) {
+      const int grow = wg_row0 + r, i = a.by_group(grow);
+      if (grow < a.rows && d < a.D)
+        store4<T>(static_cast<T*>(a.dq) + (((int64_t)b * a.Lq + i) * a.H + kv * a.G + grow - i * a.G) * a.D + d, v);
+    });
+  } else {
+    if (!there) return;
+    store_columns<T, DP>(static_cast<T*>(a.dq) + orow, dq[0], by, half, a.D);
+  }
 }
 
-template <typename T, int DP, bool KMASK>
-__global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void attn_dkv(Args a) {
-  using C = BCfg<T, DP>;
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__((BCfg<T, DP, MODE>::kThreads), (BCfg<T, DP, MODE>::kResident))
+void attn_dkv(Args a) {
+  using C = BCfg<T, DP, MODE>;
   constexpr int RT = C::kTile, RB = RT / 32;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   constexpr float kUp = kScaled ? 14.f : 0.f;
@@ -215,9 +285,14 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 
   const unsigned id = xcd_id(), bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
   const int jt = id - bkv * a.key_tiles, kv = bkv - b * a.KV;
-  const int wg_j0 = jt * kRows, j0 = wg_j0 + 32 * wave, j = j0 + (lane & 31);
+  const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
+  const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
+  const int wg_j0 = jt * C::kTileRows, j0 = wg_j0 + 32 * set, j = j0 + (lane & 31);
   const int keys = a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
-  const bool there = j < keys && (!KMASK || a.mask[(int64_t)b * a.Lk + min(j, a.Lk - 1)] != 0);
+  auto counts = [&](int key) {  // something may attend to the key
+    return key < keys && (a.mask == nullptr || a.mask[(int64_t)b * a.Lk + key] != 0);
+  };
+  const bool there = counts(j);
 
   RowOps<T, DP> k, v;
   load_rows<T, DP>(k, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)j * a.ks[1] +
@@ -229,14 +304,13 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
   int64_t rlo = 0, rhi = a.rows;
   if (a.band > 0) {
     rlo = min((int64_t)a.rows, (int64_t)wg_j0 * a.G);
-    rhi = min((int64_t)a.rows, ((int64_t)min(wg_j0 + kRows, a.Lk) - 1 + a.band) * a.G);
+    rhi = min((int64_t)a.rows, ((int64_t)min(wg_j0 + C::kTileRows, a.Lk) - 1 + a.band) * a.G);
   }
   if (wg_j0 >= keys) rhi = rlo;  // nothing attends to them: their gradients are 0
   const int tb = (int)(rlo / RT), te = rhi > rlo ? (int)((rhi + RT - 1) / RT) : tb;
 
-  const int64_t n_pad = (int64_t)a.row_tiles * kRows;
-  const float* lse = a.row_lse + ((int64_t)b * a.KV + kv) * n_pad;
-  const float* delta = a.row_delta + ((int64_t)b * a.KV + kv) * n_pad;
+  const float* lse = a.row_lse + ((int64_t)b * a.KV + kv) * a.pad_rows;
+  const float* delta = a.row_delta + ((int64_t)b * a.KV + kv) * a.pad_rows;
   int shift = 0;
   if constexpr (kScaled) {
     const float* tm = a.tile_max + ((int64_t)b * a.KV + kv) * a.row_tiles;
@@ -247,9 +321,8 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     shift = __builtin_amdgcn_readfirstlane(down(top));
   }
 
-  const unsigned lds = lds_addr(smem);
+  const unsigned lds = lds_addr(smem) + part * 2 * C::kBufKv;
   const Reads<T, DP> from(lds, lane);
-  const int wave0 = wave * 64;
   const uint64_t Q = reinterpret_cast<uint64_t>(static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)kv * a.G * a.qs[2]);
   const uint64_t GO = reinterpret_cast<uint64_t>(static_cast<const T*>(a.dout) + b * a.gs[0] + (int64_t)kv * a.G * a.gs[2]);
   // Row t RT + r is token (t RT + r) / G: where G divides RT the offsets from the tile's first token
@@ -259,29 +332,30 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
     const int token = a.by_group(row), g = row - token * a.G;
     return ((token - token0) * (unsigned)st[1] + g * (unsigned)st[2]) * (unsigned)sizeof(T);
   };
-  Stage<T, DP, RT, 256> sq, sg;
-  sq.init(tid, a.D, [&](int r) { return row_at(r, 0, a.qs); });
-  sg.init(tid, a.D, [&](int r) { return row_at(r, 0, a.gs); });
+  using SG = Stage<T, DP, RT, C::kCopiers>;
+  SG sq, sg;
+  sq.init(ctid, a.D, [&](int r) { return row_at(r, 0, a.qs); });
+  sg.init(ctid, a.D, [&](int r) { return row_at(r, 0, a.gs); });
   auto copy = [&](int t, unsigned dst) {
     const int token0 = a.by_group(t * RT);
     const uint64_t qp = Q + (uint64_t)token0 * a.qs[1] * sizeof(T), gp = GO + (uint64_t)token0 * a.gs[1] * sizeof(T);
     if (regular && (t + 1) * RT <= a.rows) {
-      sq.copy(qp, dst, wave0);
-      sg.copy(gp, dst + C::kTileBytes, wave0);
+      sq.copy(qp, dst, cwave0);
+      sg.copy(gp, dst + C::kTileBytes, cwave0);
     } else {  // rows past the end read the tile's first: their weights are 0
       auto at = [&](const int64_t* st) {
         return [=, &a](int it, unsigned o) {
-          const int r = Stage<T, DP, RT, 256>::row_of(it, tid), row = t * RT + r;
+          const int r = SG::row_of(it, ctid), row = t * RT + r;
           return o - row_at(r, 0, st) + row_at(row < a.rows ? row : t * RT, token0, st);
         };
       };
-      sq.copy(qp, dst, wave0, at(a.qs));
-      sg.copy(gp, dst + C::kTileBytes, wave0, at(a.gs));
+      sq.copy(qp, dst, cwave0, at(a.qs));
+      sg.copy(gp, dst + C::kTileBytes, cwave0, at(a.gs));
     }
     // RT logarithms, then RT deltas (the rows are padded to whole tiles there)
     const uint64_t lp = reinterpret_cast<uint64_t>(lse + t * RT), dp = reinterpret_cast<uint64_t>(delta + t * RT);
-    if (wave == 0 && lane < RT) copy4(lp, lane * 4, dst + 2 * C::kTileBytes);
-    if (wave == 1 && lane < RT) copy4(dp, lane * 4, dst + 2 * C::kTileBytes + RT * 4);
+    if ((C::kAlone || set == 0) && lane < RT) copy4(lp, lane * 4, dst + 2 * C::kTileBytes);
+    if ((C::kAlone || set == 1) && lane < RT) copy4(dp, lane * 4, dst + 2 * C::kTileBytes + RT * 4);
   };
 
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -290,14 +364,14 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
 
-  int t = tb;
+  int t = tb + part;
   if (t < te) copy(t, lds);
-  auto step = [&](auto buf) {
-    constexpr int kAt = decltype(buf)::value * C::kBuf;
-    publish();
-    if (t + 1 < te) copy(t + 1, lds + (C::kBuf - kAt));
+  auto step = [&](auto buf) __attribute__((always_inline)) {
+    constexpr int kAt = decltype(buf)::value * C::kBufKv;
+    if (C::kAlone) wait_copies(); else publish();
+    if (t + C::kParts < te) copy(t + C::kParts, lds + (C::kBufKv - kAt));
     const unsigned st = lds + kAt + 2 * C::kTileBytes;
-    if (j0 >= keys) return;
+    if (j0 >= keys || t >= te) return;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       // row r is inside key j's band iff 0 <= r - j G < band G
@@ -340,75 +414,139 @@ __global__ __launch_bounds__(256, (DP == 128 || sizeof(T) == 4 ? 1 : 2)) void at
       mma_transposed<T, DP>(dk, from, kAt, 32 * rb, ds);
     }
   };
-  while (t < te) {
+  const int end = C::kAlone ? te : te + part;
+  while (t < end) {
     step(std::integral_constant<int, 0>{});
-    if (++t >= te) break;
+    t += C::kParts;
+    if (t >= end) break;
     step(std::integral_constant<int, 1>{});
-    ++t;
+    t += C::kParts;
   }
-  if (j >= a.Lk) return;
-  const int64_t out = (((int64_t)b * a.Lk + j) * a.KV + kv) * a.D;
-  if (!there) {  // 0 whatever the zero rows that stood for the key gave
+  // a key that nothing attends to gets 0, whatever the zero row that stood for it gave
+  const float by_k = __builtin_ldexpf(a.scale, -shift), by_v = kScaled ? 0x1p-14f : 1.f;
+  if constexpr (C::kParts > 1) {
+    auto store = [&](void* to, float by) {
+      return [&, to, by](int r, int d, f32x4 v) {
+        const int key = wg_j0 + r;
+        if (key >= a.Lk || d >= a.D) return;
+        const bool some = counts(key);
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+        for (int e = 0; e < 4; ++e) v[e] = some ? v[e] * by : 0.f;
+        store4<T>(static_cast<T*>(to) + (((int64_t)b * a.Lk + key) * a.KV + kv) * a.D + d, v);
+      };
+    };
+    const unsigned base = lds_addr(smem);
+    __syncthreads();
+    join_columns<T, DP, C::kSets, C::kParts>(base, wave, lane, tid, dv, store(a.dv, by_v));
+    __syncthreads();
+    join_columns<T, DP, C::kSets, C::kParts>(base, wave, lane, tid, dk, store(a.dk, by_k));
+  } else {
+    if (j >= a.Lk) return;
+    const int64_t out = (((int64_t)b * a.Lk + j) * a.KV + kv) * a.D;
+    if (!there) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+    }
+    store_columns<T, DP>(static_cast<T*>(a.dv) + out, dv, by_v, half, a.D);
+    store_columns<T, DP>(static_cast<T*>(a.dk) + out, dk, by_k, half, a.D);
   }
-  store_columns<T, DP>(static_cast<T*>(a.dv) + out, dv, kScaled ? 0x1p-14f : 1.f, half, a.D);
-  store_columns<T, DP>(static_cast<T*>(a.dk) + out, dk, __builtin_ldexpf(a.scale, -shift), half, a.D);
 }
 
-template <typename T, int DP, bool KMASK>
-int launch(const Args& a, hipStream_t st) {
-  using C = BCfg<T, DP>;
-  static std::atomic<unsigned long long> done_q{0}, done_kv{0};
-  const int dev = stream_device(st);
-  if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK>), C::kLdsQ, dev, done_q)) return rc;
-  if (const int rc = ensure_lds_limit(reinterpret_cast<const void*>(&attn_dkv<T, DP, KMASK>), C::kLdsKv, dev, done_kv)) return rc;
-  const int64_t bkv = (int64_t)a.B * a.KV, key_tiles = a.key_tiles;
-  if (bkv * a.row_tiles > 0x7fffffffll || bkv * key_tiles > 0x7fffffffll)
+template <typename T, int DP, bool KMASK, int MODE>
+int launch_dq(Args a, hipStream_t st) {
+  using C = BCfg<T, DP, MODE>;
+  static std::atomic<unsigned long long> done{0};
+  const void* kern = reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK, MODE>);
+  if (const int rc = ensure_lds_limit(kern, C::kLdsQ, stream_device(st), done)) return rc;
+  const int64_t grid = (int64_t)a.B * a.KV * a.row_tiles;
+  attn_dq<T, DP, KMASK, MODE><<<dim3((unsigned)grid), C::kThreads, C::kLdsQ, st>>>(a);
+  return check_launch("cross_attention_backward dq");
+}
+
+template <typename T, int DP, int MODE>
+int launch_dkv(Args a, hipStream_t st) {
+  using C = BCfg<T, DP, MODE>;
+  static std::atomic<unsigned long long> done{0};
+  const void* kern = reinterpret_cast<const void*>(&attn_dkv<T, DP, MODE>);
+  if (const int rc = ensure_lds_limit(kern, C::kLdsKv, stream_device(st), done)) return rc;
+  a.key_tiles = (int)ceil_div(a.Lk, C::kTileRows);
+  a.by_key_tiles = Divide(a.key_tiles);
+  const int64_t grid = (int64_t)a.B * a.KV * a.key_tiles;
+  attn_dkv<T, DP, MODE><<<dim3((unsigned)grid), C::kThreads, C::kLdsKv, st>>>(a);
+  return check_launch("cross_attention_backward dk, dv");
+}
+
+// `wgs`: workgroups of 128 rows.  Up to a quarter of the compute units: 32-row workgroups; up to one
+// each: eight waves (up to half and 32-row workgroups where eight do not fit)
+int mode_of(int64_t wgs, bool has_some, bool has_few) {
+  if (!has_few) return kMany;
+  if (wgs <= kCus / 4) return kFewRows;
+  if (has_some) return wgs <= kCus ? kSome : kMany;
+  return wgs <= kCus / 2 ? kFewRows : kMany;
+}
+
+template <typename T, int DP>
+int launch(Args a, hipStream_t st) {
+  const int64_t bkv = (int64_t)a.B * a.KV;
+  if (bkv * (a.pad_rows / 32) > 0x7fffffffll || bkv * ceil_div(a.Lk, 32) > 0x7fffffffll)
     return fail(SM_EINVAL, "cross_attention_backward: too many row tiles");
+  constexpr bool some = BCfg<T, DP, kMany>::kHasSome;
+  a.row_tiles = a.pad_rows / kRows;
   if (a.row_tiles > 0) {
-    attn_dq<T, DP, KMASK><<<dim3((unsigned)(bkv * a.row_tiles)), 256, C::kLdsQ, st>>>(a);
-    if (const int rc = check_launch("cross_attention_backward dq")) return rc;
+    const int mode = mode_of(bkv * a.row_tiles, some, true);
+    if (mode == kFewRows) a.row_tiles = a.pad_rows / 32;
+    a.by_row_tiles = Divide(a.row_tiles);
+    const bool km = a.mask != nullptr;
+    int rc = SM_OK;
+    if (mode == kFewRows)
+      rc = km ? launch_dq<T, DP, true, kFewRows>(a, st) : launch_dq<T, DP, false, kFewRows>(a, st);
+    else if (mode == kMany)
+      rc = km ? launch_dq<T, DP, true, kMany>(a, st) : launch_dq<T, DP, false, kMany>(a, st);
+    else if constexpr (some)
+      rc = km ? launch_dq<T, DP, true, kSome>(a, st) : launch_dq<T, DP, false, kSome>(a, st);
+    if (rc) return rc;
   }
-  if (key_tiles > 0) {
-    attn_dkv<T, DP, KMASK><<<dim3((unsigned)(bkv * key_tiles)), 256, C::kLdsKv, st>>>(a);
-    return check_launch("cross_attention_backward dk, dv");
+  if (a.Lk > 0 && bkv > 0) {
+    // (32 wide fp32 keys in each of two waves would not fit their registers)
+    constexpr bool few = sizeof(T) == 2 || DP < 128;
+    const int mode = mode_of(bkv * ceil_div(a.Lk, kRows), some, few);
+    if constexpr (few)
+      if (mode == kFewRows) return launch_dkv<T, DP, kFewRows>(a, st);
+    if (mode == kMany) return launch_dkv<T, DP, kMany>(a, st);
+    if constexpr (some) return launch_dkv<T, DP, kSome>(a, st);
   }
   return SM_OK;
 }
 
 template <typename T>
 int by_width(const Args& a, hipStream_t st) {
-  const bool km = a.mask != nullptr;
-  if (a.D <= 32) return km ? launch<T, 32, true>(a, st) : launch<T, 32, false>(a, st);
-  if (a.D <= 64) return km ? launch<T, 64, true>(a, st) : launch<T, 64, false>(a, st);
-  return km ? launch<T, 128, true>(a, st) : launch<T, 128, false>(a, st);
+  if (a.D <= 32) return launch<T, 32>(a, st);
+  if (a.D <= 64) return launch<T, 64>(a, st);
+  return launch<T, 128>(a, st);
 }
 
 }  // namespace
 
+// per row its logarithm and delta, and room for a maximum of each 32 rows
 int64_t bwd_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV) {
   if (B <= 0 || Lq <= 0 || H <= 0 || KV <= 0 || H % KV != 0) return 0;
-  const int64_t tiles = ceil_div(Lq * (H / KV), kRows);
-  return B * KV * tiles * (2 * kRows + 1) * 4;
+  const int64_t pad = ceil_div(Lq * (H / KV), kRows) * kRows;
+  return B * KV * (2 * pad + pad / 32) * 4;
 }
 
 int bwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st) {
-  a.row_tiles = (int)ceil_div(a.rows, kRows);
-  const int64_t n = (int64_t)a.B * a.KV * a.row_tiles;
-  if (n > 0 && (workspace == nullptr || ws_bytes < n * (2 * kRows + 1) * 4))
+  a.pad_rows = (int)(ceil_div(a.rows, kRows) * kRows);
+  const int64_t n = (int64_t)a.B * a.KV * a.pad_rows;
+  if (n > 0 && (workspace == nullptr || ws_bytes < (2 * n + n / 32) * 4))
     return fail(SM_EINVAL, "cross_attention_backward: the workspace is smaller than "
                            "sm_cross_attention_backward_workspace_bytes()");
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return fail(SM_EINVAL, "cross_attention_backward: the workspace must be 16-byte aligned");
   a.row_lse = static_cast<float*>(workspace);
-  a.row_delta = a.row_lse + n * kRows;
-  a.tile_max = a.row_delta + n * kRows;
-  a.key_tiles = (int)ceil_div(a.Lk, kRows);
-  a.by_row_tiles = Divide(a.row_tiles);
-  a.by_key_tiles = Divide(a.key_tiles);
+  a.row_delta = a.row_lse + n;
+  a.tile_max = a.row_delta + n;
   SM_DISPATCH_DTYPE(dtype, T, return by_width<T>(a, st));
   return SM_OK;
 }

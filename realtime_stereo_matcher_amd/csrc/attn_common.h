@@ -55,8 +55,9 @@ struct Args {
   int64_t qs[3], ks[3], vs[3], gs[3];  // element strides of batch, token and head
   int B, Lq, Lk, H, KV, G, D;
   int rows, row_tiles;    // Lq * G and its tiles: row r is token r / G, head kv * G + r % G
+  int pad_rows;           // rows up to a multiple of 128 (backward)
   int band;               // > 0: key j is a candidate of token i iff 0 <= i - j < band
-  int splits, key_tiles;  // of 128 keys (backward)
+  int splits, key_tiles;  // shares of the keys; tiles of keys (backward)
   Divide by_group, by_kv, by_row_tiles, by_splits, by_key_tiles;
   float scale, c;         // c = scale * log2(e): exp(scale x) = exp2(c x)
 };
@@ -110,7 +111,13 @@ __device__ __forceinline__ void lds_put(unsigned addr, V v) {
 // lane, without a register in between.  Inline, because the compiler would wait for every such copy
 // in flight before each LDS read; the kernels wait themselves (wait_copies, publish) before a tile is
 // read.
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)x) |
+         (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
 __device__ __forceinline__ void copy16(uint64_t base, unsigned off, unsigned dst) {
+  base = uniform(base);
+  dst = __builtin_amdgcn_readfirstlane(dst);
   unsigned keep;
   asm volatile(
       "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\t"
@@ -120,6 +127,8 @@ __device__ __forceinline__ void copy16(uint64_t base, unsigned off, unsigned dst
       : "memory");
 }
 __device__ __forceinline__ void copy4(uint64_t base, unsigned off, unsigned dst) {
+  base = uniform(base);
+  dst = __builtin_amdgcn_readfirstlane(dst);
   unsigned keep;
   asm volatile(
       "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %2, %1\n\t"
@@ -197,17 +206,22 @@ template <typename T, int DP, int ROWS, int NT> struct Stage {
 template <typename T, int DP> struct Reads {
   using TL = Tile<T, DP>;
   static constexpr bool kWide = sizeof(T) == 4;
-  unsigned row[kWide ? 1 : TL::kSteps], col[kWide ? 1 : DP / 32][2];
-  int lane;
-  __device__ __forceinline__ Reads(unsigned lds, int lane_) : lane(lane_) {
-    const int half = lane >> 5;
-    if constexpr (kWide) {
-      row[0] = lds;
-    } else {
-      const int r = lane & 31;
+  static constexpr int kRowRegs = TL::kSteps < 8 ? TL::kSteps : 8;  // twists are less than 16 pieces
+  typedef float Columns __attribute__((ext_vector_type(DP / 32)));  // fp32: one of each block
+  unsigned row[kRowRegs], col[kWide ? 8 : DP / 16];
+  __device__ __forceinline__ Reads(unsigned lds, int lane) {
+    const int half = lane >> 5, r = lane & 31;
 #pragma unroll
-      for (int c = 0; c < TL::kSteps; ++c)
-        row[c] = lds + r * TL::kRowBytes + ((2 * c + half) ^ TL::twist(r)) * 16;
+    for (int c = 0; c < kRowRegs; ++c)
+      row[c] = lds + r * TL::kRowBytes + ((2 * c + half) ^ TL::twist(r)) * 16;
+    if constexpr (kWide) {
+      // lane m's columns are the DP / 32 neighbours from (DP / 32) m on, one of each block
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int q = 8 * (u >> 2) + 4 * half + (u & 3), at = r * (DP / 8);
+        col[u] = lds + q * TL::kRowBytes + (((at >> 4) ^ TL::twist(q)) << 4) + (at & 15);
+      }
+    } else {
       // ds_read_tr16_b64: in each 16 lanes, lane i receives column i of the 4 x 16 values whose row
       // j the lanes 4j .. 4j+3 address
       const int g = (lane >> 4) & 1, l16 = lane & 15;
@@ -216,19 +230,14 @@ template <typename T, int DP> struct Reads {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int q = 8 * u + 4 * half + (l16 >> 2);
-          col[db][u] = lds + q * TL::kRowBytes +
-                       ((4 * db + 2 * g + ((l16 & 3) >> 1)) ^ TL::twist(q)) * 16 + (l16 & 1) * 8;
+          col[2 * db + u] = lds + q * TL::kRowBytes +
+                            ((4 * db + 2 * g + ((l16 & 3) >> 1)) ^ TL::twist(q)) * 16 + (l16 & 1) * 8;
         }
     }
   }
   // left operand with the tile's rows as its rows: rows row0 .. row0+31 (row0 a multiple of 32), step c
   __device__ __forceinline__ Frag<T> rows(int tile, int row0, int c) const {
-    if constexpr (kWide) {
-      const int r = lane & 31, ch = (2 * c + (lane >> 5)) ^ TL::twist(r);
-      return lds_get<Frag<T>>(row[0] + tile + (row0 + r) * TL::kRowBytes + ch * 16);
-    } else {
-      return lds_get<Frag<T>>(row[c] + (tile + row0 * TL::kRowBytes));
-    }
+    return lds_get<Frag<T>>(row[c % kRowRegs] + (tile + row0 * TL::kRowBytes + c / kRowRegs * 256));
   }
   // the same transposed, 16-bit: rows row0 + 16 s .. + 15 as the contraction of column block db
   __device__ __forceinline__ Frag<T> columns(int tile, int row0, int s, int db) const {
@@ -236,19 +245,36 @@ template <typename T, int DP> struct Reads {
     typedef __attribute__((address_space(3))) s16x4 lds_s4;
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const unsigned at = tile + (row0 + 16 * s) * TL::kRowBytes;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[db][0] + at));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[db][1] + at));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[2 * db] + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>(col[2 * db + 1] + at));
     const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(Frag<T>, both);
   }
-  // fp32: row `row0 + crow(r)` of the tile, a lane's column of block db
-  __device__ __forceinline__ float column(int tile, int row0, int r, int db) const {
+  // fp32: the lane's columns of row `row0` + 8 (r/4) + 4 half + r%4
+  __device__ __forceinline__ Columns columns(int tile, int row0, int r) const {
     static_assert(kWide, "fp32");
-    const int c = lane & 31, q = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    const int ch = (8 * db + (c >> 2)) ^ TL::twist(q);
-    return lds_get<float>(row[0] + tile + q * TL::kRowBytes + ch * 16 + (c & 3) * 4);
+    return lds_get<Columns>(col[r & 7] + (tile + (row0 + 16 * (r >> 3)) * TL::kRowBytes));
   }
 };
+
+// A lane's part of a transposed result, as DP / 8 vectors of 4 neighbouring columns of its row.
+template <typename T, int DP>
+__device__ __forceinline__ int column_at(int i, int half) {
+  if constexpr (sizeof(T) == 4 && DP > 32) {  // the order of Reads::columns
+    const int r = DP == 64 ? 2 * i : i;
+    return (DP / 32) * (8 * (r >> 2) + 4 * half + (r & 3));
+  }
+  return 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
+}
+template <typename T, int DP>
+__device__ __forceinline__ f32x4 column_values(const f32x16 (&acc)[DP / 32], int i) {
+  if constexpr (sizeof(T) == 4 && DP == 128) return f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+  if constexpr (sizeof(T) == 4 && DP == 64)
+    return f32x4{acc[0][2 * i], acc[1][2 * i], acc[0][2 * i + 1], acc[1][2 * i + 1]};
+  const f32x16& b = acc[i >> 2];
+  const int g = 4 * (i & 3);
+  return f32x4{b[g], b[g + 1], b[g + 2], b[g + 3]};
+}
 
 // acc[n][db] += (tile rows row0 .. row0+31, transposed) * block[n], where a block holds a 32x32
 // result (tile rows x lane columns): values of the tile's column are the rows of the product.  N
@@ -258,14 +284,14 @@ __device__ __forceinline__ void mma_transposed(f32x16 (&acc)[N][DP / 32], const 
                                                int tile, int row0, const f32x16 (&block)[N]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < 16; ++r) {
+      const auto a = from.columns(tile, row0, r);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) {
-        const float a = from.column(tile, row0, r, db);
+      for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
         for (int n = 0; n < N; ++n)
-          acc[n][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, block[n][r], acc[n][db], 0, 0, 0);
-      }
+          acc[n][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[db], block[n][r], acc[n][db], 0, 0, 0);
+    }
   } else {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -400,19 +426,15 @@ template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 v) {
   }
 }
 
-// a lane's column of the transposed result to its row in memory: 4 values a store
-template <typename T, int DP>
-__device__ __forceinline__ void store_columns(T* row, const f32x16 (&acc)[DP / 32], float by,
+// a lane's column of the transposed result of type-T operands to its row in memory (S: stored type)
+template <typename T, int DP, typename S = T>
+__device__ __forceinline__ void store_columns(S* row, const f32x16 (&acc)[DP / 32], float by,
                                               int half, int D) {
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * db + 8 * g + 4 * half;
-      if (d < D)
-        store4<T>(row + d, f32x4{acc[db][4 * g] * by, acc[db][4 * g + 1] * by,
-                                 acc[db][4 * g + 2] * by, acc[db][4 * g + 3] * by});
-    }
+  for (int i = 0; i < DP / 8; ++i) {
+    const int d = column_at<T, DP>(i, half);
+    if (d < D) store4<S>(row + d, column_values<T, DP>(acc, i) * by);
+  }
 }
 
 // Workgroups go to the 8 XCDs in turn; neighbours in `id` share keys and values, so each XCD gets

@@ -17,8 +17,8 @@ namespace attn {
 namespace {
 
 // How the waves of a workgroup share the work:
-//   FEW       at most 32 query rows (single tokens with shared heads): all waves hold the same rows and
-//             take the key tiles in turn, each with its own LDS and without barriers
+//   FEW       32 query rows (single tokens with shared heads, short launches): all waves hold the same
+//             rows and take the key tiles in turn, each with its own LDS and without barriers
 //   GROUPS    1: four waves, 32 rows each; 2: eight waves, 32 rows for each pair, which takes the even
 //             and the odd key tiles
 // Waves that hold the same rows join their sums and statistics through LDS at the end.
@@ -106,7 +106,7 @@ void attn_fwd(Args a) {
   }
   if (KMASK) byte = keys.byte(t + kStep, lane);
 
-  auto step = [&](auto buf) {
+  auto step = [&](auto buf) __attribute__((always_inline)) {
     constexpr int kBuf = decltype(buf)::value * C::kBufBytes;
     // this tile is in LDS, and nobody reads the other buffer any more
     if (FEW) wait_copies(); else publish();
@@ -180,11 +180,8 @@ void attn_fwd(Args a) {
     __syncthreads();
     const unsigned mine = base + wave * kWaveBytes;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        lds_put(mine + (lane & 31) * kPitch + (32 * db + 8 * g + 4 * half) * 4,
-                f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]});
+    for (int i = 0; i < DP / 8; ++i)
+      lds_put(mine + (lane & 31) * kPitch + column_at<T, DP>(i, half) * 4, column_values<T, DP>(o, i));
     if (half == 0) {
       lds_put(mine + 32 * kPitch + lane * 4, m);
       lds_put(mine + 32 * kPitch + 128 + lane * 4, l);
@@ -234,7 +231,7 @@ void attn_fwd(Args a) {
     const float lse = l == 0.f ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l)) * kLn2;
     if (a.splits > 1) {
       const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + at;
-      store_columns<float, DP>(a.part_o + ps * a.D, o, inv, half, a.D);
+      store_columns<T, DP, float>(a.part_o + ps * a.D, o, inv, half, a.D);
       if (half == 0) a.part_l[ps] = lse;
     } else {
       store_columns<T, DP>(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + token) * a.H + head) * a.D,
@@ -275,6 +272,12 @@ __global__ __launch_bounds__(256) void attn_join(Args a) {
   if (d == 0 && a.lse) a.lse[r] = sum == 0.f ? -INFINITY : base + __builtin_amdgcn_logf(sum) * kLn2;
 }
 
+// 32-row workgroups whose waves split the keys: a single tile of rows, or a launch whose 128-row
+// workgroups would fill no more than a quarter of the compute units
+bool few_rows(int64_t B, int64_t KV, int64_t rows) {
+  return rows <= kFew || B * KV * ceil_div(rows, kRows) <= kCus / 4;
+}
+
 template <typename T, int DP, bool KMASK, bool FEW, int GROUPS>
 int launch(const Args& a, hipStream_t st) {
   using C = Cfg<T, DP, FEW, GROUPS>;
@@ -295,7 +298,7 @@ int launch(const Args& a, hipStream_t st) {
 
 template <typename T, int DP, bool KMASK>
 int by_rows(const Args& a, hipStream_t st) {
-  if (a.rows <= kFew) return launch<T, DP, KMASK, true, 1>(a, st);
+  if (few_rows(a.B, a.KV, a.rows)) return launch<T, DP, KMASK, true, 1>(a, st);
   // a launch that leaves a compute unit one workgroup gives it eight waves instead of four (wide fp32
   // rows need the registers of four)
   if constexpr (sizeof(T) == 2 || DP < 128) {
@@ -317,7 +320,7 @@ int by_width(const Args& a, hipStream_t st) {
 // once, at least 256 keys each (below that the join costs more than the split gains).
 int split_count(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV) {
   const int64_t rows = Lq * (H / KV);
-  const int64_t wgs = B * KV * ceil_div(rows, rows <= kFew ? kFew : kRows);
+  const int64_t wgs = B * KV * ceil_div(rows, few_rows(B, KV, rows) ? kFew : kRows);
   const int64_t s = std::min<int64_t>(kCus / std::max<int64_t>(wgs, 1), Lk / 256);
   return (int)std::max<int64_t>(1, s);
 }
@@ -376,7 +379,7 @@ int64_t fwd_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_
 
 int fwd_entry(Args& a, int dtype, void* workspace, int64_t ws_bytes, hipStream_t st) {
   a.splits = split_count(a.B, a.Lq, a.Lk, a.H, a.KV);
-  a.row_tiles = (int)ceil_div(a.rows, a.rows <= kFew ? kFew : kRows);
+  a.row_tiles = (int)ceil_div(a.rows, few_rows(a.B, a.KV, a.rows) ? kFew : kRows);
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.splits * a.B * a.H * a.Lq;
     if (workspace == nullptr || ws_bytes < n * (a.D + 1) * 4)
