@@ -50,8 +50,14 @@ void attn_fwd(Args a) {
   const int ctid = FEW ? lane : tid & 255, cwave0 = FEW ? 0 : (wave & 3) * 64;
 
   const unsigned id = xcd_id();
-  const unsigned by_tile = a.by_row_tiles(id), by_split = a.by_splits(by_tile), b = a.by_kv(by_split);
-  const int rt = id - by_tile * a.row_tiles, split = by_tile - by_split * a.splits, kv = by_split - b * a.KV;
+  // neighbours share the keys of a head, or (few rows) read the same tokens of neighbouring heads
+  const unsigned u = FEW ? a.by_kv(id) : a.by_row_tiles(id);
+  const int in_u = id - u * (FEW ? a.KV : a.row_tiles);
+  const unsigned w = FEW ? a.by_row_tiles(u) : a.by_splits(u);
+  const int in_w = u - w * (FEW ? a.row_tiles : a.splits);
+  const unsigned b = FEW ? a.by_splits(w) : a.by_kv(w);
+  const int in_b = w - b * (FEW ? a.splits : a.KV);
+  const int rt = FEW ? in_w : in_u, split = FEW ? in_b : in_w, kv = FEW ? in_u : in_b;
 
   const int wg_row0 = rt * kTileRows;
   const int row0 = wg_row0 + (FEW ? 0 : 32 * (wave & 3));  // of this wave
@@ -251,17 +257,37 @@ __global__ __launch_bounds__(256) void attn_join(Args a) {
   if (p >= n * per) return;
   const int64_t r = p / per;
   const int d = 4 * (int)(p % per);
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_l[s * n + r]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
+  constexpr int kAtOnce = 8;  // splits whose loads are in flight together
+  float top = -INFINITY, base = 0.f, sum = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f((a.part_l[s * n + r] - base) * kLog2e);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (s * n + r) * a.D + d);
-    sum += w;
+  for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
+    float l[kAtOnce];
+    f32x4 x[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(w, x[e], v[e]);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = (int64_t)min(s0 + i, a.splits - 1) * n + r;
+      l[i] = a.part_l[at];
+      x[i] = *reinterpret_cast<const f32x4*>(a.part_o + at * a.D + d);
+    }
+    float most = top;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (s0 + i >= a.splits) l[i] = -INFINITY;
+      most = fmaxf(most, l[i]);
+    }
+    base = most == -INFINITY ? 0.f : most;
+    const float keep = __builtin_amdgcn_exp2f((top - base) * kLog2e);
+    top = most;
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float w = __builtin_amdgcn_exp2f((l[i] - base) * kLog2e);
+      sum += w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(w, x[i][e], v[e]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll

@@ -606,6 +606,7 @@ def warp_by_flow_map(image, flow):
 
 
 # ------------------------------------------------------------------- matching by attention
+_POSITIONS = (torch.int32, torch.int64)
 _TOKEN_DTYPES = {torch.float32: _lib.SM_F32, torch.float16: _lib.SM_F16, torch.bfloat16: _lib.SM_BF16}
 
 
@@ -618,18 +619,27 @@ def _token_dtype(t, what, name):
 
 
 def _tensors(what, *named):
-    for name, t in zip(named[::2], named[1::2]):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{what}: {name} must be a tensor")
+    for i in range(1, len(named), 2):
+        if not isinstance(named[i], torch.Tensor):
+            raise TypeError(f"{what}: {named[i - 1]} must be a tensor")
+
+
+def _one_device(*ts):
+    """The index of the tensors' HIP device; _device_check's errors."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index or index < 0:
+            _device_check(*ts)
+    return index
 
 
 def _on_device(fn):
-    """Run ``fn(dev, ...)`` with ``dev`` the current device (where its launches go)."""
-    def run(dev, *args):
-        if torch.cuda.current_device() == dev.index:
-            return fn(dev, *args)
-        with torch.cuda.device(dev):
-            return fn(dev, *args)
+    """Run ``fn(index, ...)`` with device ``index`` the current one (where its launches go)."""
+    def run(index, *args):
+        if torch.cuda.current_device() == index:
+            return fn(index, *args)
+        with torch.cuda.device(index):
+            return fn(index, *args)
     return run
 
 
@@ -653,7 +663,7 @@ def _grads_wanted(*ts):
 
 
 @_on_device
-def _attention_forward(dev, q, k, v, lengths, mask, scale, band, want_lse):
+def _attention_forward(index, q, k, v, lengths, mask, scale, band, want_lse):
     b, lq, h, d = q.shape
     lk, kv = k.shape[1], k.shape[2]
     out = q.new_empty((b, lq, h, d))
@@ -669,12 +679,12 @@ def _attention_forward(dev, q, k, v, lengths, mask, scale, band, want_lse):
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
             _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, qs, ks, vs, scale, band,
             None if lengths is None else lengths.data_ptr(), None if mask is None else mask.data_ptr(),
-            ws.data_ptr() if nws else None, nws, _raw_stream(dev.index)), "sm_cross_attention")
+            ws.data_ptr() if nws else None, nws, _raw_stream(index)), "sm_cross_attention")
     return out, lse
 
 
 @_on_device
-def _attention_backward(dev, q, k, v, out, lse, dout, lengths, mask, scale, band):
+def _attention_backward(index, q, k, v, out, lse, dout, lengths, mask, scale, band):
     b, lq, h, d = q.shape
     lk, kv = k.shape[1], k.shape[2]
     dq = q.new_empty((b, lq, h, d))
@@ -694,14 +704,14 @@ def _attention_backward(dev, q, k, v, out, lse, dout, lengths, mask, scale, band
             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _TOKEN_DTYPES[q.dtype], b, lq, lk, h, kv, d, qs, ks,
             vs, gs, scale, band, None if lengths is None else lengths.data_ptr(),
             None if mask is None else mask.data_ptr(), ws.data_ptr() if nws else None, nws,
-            _raw_stream(dev.index)), "sm_cross_attention_backward")
+            _raw_stream(index)), "sm_cross_attention_backward")
     return dq, dk, dv
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale, band):
-        out, lse = _attention_forward(q.device, q, k, v, lengths, mask, scale, band, True)
+        out, lse = _attention_forward(q.get_device(), q, k, v, lengths, mask, scale, band, True)
         ctx.save_for_backward(q, k, v, out, lse, lengths, mask)
         ctx.scale, ctx.band = scale, band
         ctx.mark_non_differentiable(lse)
@@ -711,21 +721,22 @@ class _CrossAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, _):
         q, k, v, out, lse, lengths, mask = ctx.saved_tensors
-        return (*_attention_backward(q.device, q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
+        return (*_attention_backward(q.get_device(), q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
                 None, None, None, None)
 
 
 def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_mask):
     what = "cross_attention"
     _tensors(what, "query", query, "key", key, "value", value)
-    if query.dim() != 4 or key.dim() != 4:
-        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(query.shape)} and "
-                           f"{tuple(key.shape)}")
-    if key.shape != value.shape:
-        raise RuntimeError(f"{what}: key/value shape mismatch {tuple(key.shape)} vs {tuple(value.shape)}")
-    b, lq, h, d = query.shape
-    lk, kv = key.shape[1], key.shape[2]
-    if key.shape[0] != b or key.shape[3] != d:
+    qshape, kshape = query.shape, key.shape
+    if len(qshape) != 4 or len(kshape) != 4:
+        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(qshape)} and "
+                           f"{tuple(kshape)}")
+    if kshape != value.shape:
+        raise RuntimeError(f"{what}: key/value shape mismatch {tuple(kshape)} vs {tuple(value.shape)}")
+    b, lq, h, d = qshape
+    kb, lk, kv, kd = kshape
+    if kb != b or kd != d:
         raise RuntimeError(f"{what}: query {tuple(query.shape)} and key {tuple(key.shape)} differ in batch "
                            "or head width")
     if (h % kv if kv else h) != 0:
@@ -753,14 +764,16 @@ def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_
         if key_mask.shape != (b, lk) or key_mask.dtype != torch.bool:
             raise RuntimeError(f"{what}: key_mask must be ({b}, {lk}) truth values, got "
                                f"{tuple(key_mask.shape)} {key_mask.dtype}")
-    _device_check(*(t for t in (query, key, value, key_lengths, key_mask) if t is not None))
+    index = _one_device(query, key, value)
     if key_lengths is not None:
+        _one_device(query, key_lengths)
         if key_lengths.dtype == torch.int64:
             key_lengths = key_lengths.clamp(0, lk).to(torch.int32)
         key_lengths = key_lengths.contiguous()
     if key_mask is not None:
+        _one_device(query, key_mask)
         key_mask = key_mask.contiguous()
-    return scale, band, key_lengths, key_mask
+    return index, scale, band, key_lengths, key_mask
 
 
 def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengths=None,
@@ -790,12 +803,12 @@ def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengt
     if _traced():
         out, lse = _ops().cross_attention(query, key, value, key_lengths, key_mask, scale, max_disparity)
     else:
-        scale, band, lengths, mask = _attention_checks(query, key, value, scale, max_disparity,
-                                                       key_lengths, key_mask)
+        index, scale, band, lengths, mask = _attention_checks(query, key, value, scale, max_disparity,
+                                                              key_lengths, key_mask)
         if _grads_wanted(query, key, value):
             out, lse = _CrossAttention.apply(query, key, value, lengths, mask, scale, band)
         else:
-            out, lse = _attention_forward(query.device, query, key, value, lengths, mask, scale, band, return_lse)
+            out, lse = _attention_forward(index, query, key, value, lengths, mask, scale, band, return_lse)
     if not return_lse:
         return out
     b, lq, h, _ = query.shape
@@ -841,24 +854,25 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_len
 
 
 @_on_device
-def _rotary_run(dev, x, positions, frequencies, interleaved, amplitude, inverse):
-    b, l, h, d = x.shape
-    y = x.new_empty((b, l, h, d))
-    if y.numel():
+def _rotary_run(index, x, positions, frequencies, interleaved, amplitude, inverse):
+    b, l, h, d = shape = x.shape
+    y = x.new_empty(shape)
+    if b and l and h:
         st = None
         if not x.is_contiguous():
             if x.stride(3) != 1 and d > 1:
                 x = x.contiguous()
             else:
-                st = _lib.int64s(*(0 if n == 1 else s for n, s in zip(x.shape[:3], x.stride())))
+                st = _lib.int64s(*(0 if n == 1 else s for n, s in zip(shape, x.stride()[:3])))
         flags = ((_lib.SM_ROTARY_INTERLEAVED if interleaved else 0)
                  | (_lib.SM_ROTARY_INVERSE if inverse else 0)
                  | (_lib.SM_ROTARY_POS64 if positions.dtype == torch.int64 else 0))
-        ps = positions.stride(0) if positions.dim() == 2 and b > 1 else 0
-        _lib.check(_lib.load().sm_rotary(
+        ps = positions.stride(0) if b > 1 and positions.dim() == 2 else 0
+        rc = _lib.load().sm_rotary(
             x.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), y.data_ptr(), _TOKEN_DTYPES[x.dtype],
-            b, l, h, d, 2 * frequencies.numel(), st, ps, flags, amplitude, _raw_stream(dev.index)),
-            "sm_rotary")
+            b, l, h, d, 2 * frequencies.shape[0], st, ps, flags, amplitude, _raw_stream(index))
+        if rc:
+            _lib.check(rc, "sm_rotary")
     return y
 
 
@@ -867,12 +881,12 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, frequencies, interleaved, amplitude):
         ctx.save_for_backward(positions, frequencies)
         ctx.how = interleaved, amplitude
-        return _rotary_run(x.device, x, positions, frequencies, interleaved, amplitude, False)
+        return _rotary_run(x.get_device(), x, positions, frequencies, interleaved, amplitude, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return (_rotary_run(dy.device, dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
+        return (_rotary_run(dy.get_device(), dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
 
 
 def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
@@ -889,30 +903,33 @@ def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
         return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
     what = "rotary"
     _tensors(what, "x", x, "positions", positions, "frequencies", frequencies)
-    if x.dim() != 4:
-        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(x.shape)}")
+    shape, pshape = x.shape, positions.shape
+    if len(shape) != 4:
+        raise RuntimeError(f"{what}: expected (B, L, heads, D) tokens, got {tuple(shape)}")
     _token_dtype(x, what, "x")
-    b, l, _, d = x.shape
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((l,), (b, l)):
+    b, l, _, d = shape
+    if (positions.dtype not in _POSITIONS or pshape[-1:] != (l,)
+            or not (len(pshape) == 1 or (len(pshape) == 2 and pshape[0] == b))):
         raise RuntimeError(f"{what}: positions must be ({l},) or ({b}, {l}) int32 or int64, got "
-                           f"{tuple(positions.shape)} {positions.dtype}")
+                           f"{tuple(pshape)} {positions.dtype}")
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
         raise RuntimeError(f"{what}: frequencies must be one row of float64, got "
                            f"{tuple(frequencies.shape)} {frequencies.dtype}")
-    if not 2 <= 2 * frequencies.numel() <= d:
-        raise RuntimeError(f"{what}: {frequencies.numel()} pairs do not fit heads of {d} values")
+    if not 2 <= 2 * frequencies.shape[0] <= d:
+        raise RuntimeError(f"{what}: {frequencies.shape[0]} pairs do not fit heads of {d} values")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"{what}: layout must be 'half' or 'interleaved'")
     if frequencies.requires_grad:
         raise RuntimeError(f"{what}: frequencies have no gradient")
-    _device_check(x, positions, frequencies)
+    index = _one_device(x, positions, frequencies)
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    frequencies = frequencies.contiguous()
-    how = layout == "interleaved", float(amplitude)
-    if _grads_wanted(x):
-        return _Rotary.apply(x, positions, frequencies, *how)
-    return _rotary_run(x.device, x, positions, frequencies, *how, False)
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
+    interleaved, amplitude = layout == "interleaved", float(amplitude)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, positions, frequencies, interleaved, amplitude)
+    return _rotary_run(index, x, positions, frequencies, interleaved, amplitude, False)
 
 
 # ------------------------------------------------------------------------------------- RMS norm
@@ -930,56 +947,60 @@ def _norm_checks(what, x, weight, residual, eps):
     _tensors(what, "x", x, "weight", weight)
     if residual is not None:
         _tensors(what, "residual", residual)
-    if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
-        raise RuntimeError(f"{what}: expected (..., C) rows and (C,) weight, got {tuple(x.shape)} and "
+    shape, dtype = x.shape, x.dtype
+    if weight.dim() != 1 or shape[-1:] != weight.shape:
+        raise RuntimeError(f"{what}: expected (..., C) rows and (C,) weight, got {tuple(shape)} and "
                            f"{tuple(weight.shape)}")
-    if not 1 <= x.shape[-1] <= 65536:
-        raise RuntimeError(f"{what}: rows of 1 to 65536 values, got {x.shape[-1]}")
+    if not 1 <= shape[-1] <= 65536:
+        raise RuntimeError(f"{what}: rows of 1 to 65536 values, got {shape[-1]}")
     _token_dtype(x, what, "x")
-    for name, t in (("weight", weight), ("residual", residual)):
-        if t is not None and t.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"{what}: {name} must be {x.dtype} or float32, got {t.dtype}")
-    if residual is not None and residual.shape != x.shape:
-        raise RuntimeError(f"{what}: x/residual shape mismatch {tuple(x.shape)} vs {tuple(residual.shape)}")
+    if weight.dtype not in (dtype, torch.float32):
+        raise TypeError(f"{what}: weight must be {dtype} or float32, got {weight.dtype}")
+    if residual is not None:
+        if residual.dtype not in (dtype, torch.float32):
+            raise TypeError(f"{what}: residual must be {dtype} or float32, got {residual.dtype}")
+        if residual.shape != shape:
+            raise RuntimeError(f"{what}: x/residual shape mismatch {tuple(shape)} vs {tuple(residual.shape)}")
     if not 0.0 <= float(eps) < 3.4e38:
         raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
-    if residual is None:
-        _device_check(x, weight)
-    else:
-        _device_check(x, weight, residual)
+    return _one_device(x, weight) if residual is None else _one_device(x, weight, residual)
 
 
 @_on_device
-def _norm_forward(dev, x, weight, residual, eps, e4m3=None):
+def _norm_forward(index, x, weight, residual, eps, e4m3=None):
     """(y, summed or None), or with ``e4m3`` (the group) (q, scales, summed or None)."""
-    c = x.shape[-1]
     shape, code = x.shape, _TOKEN_DTYPES[x.dtype]
+    c = shape[-1]
     summed = None if residual is None else residual.new_empty(shape)
-    y = x.new_empty(shape, dtype=x.dtype if e4m3 is None else torch.float8_e4m3fn)
-    scales = None
-    if e4m3 is not None:
+    if e4m3 is None:
+        y, scales = x.new_empty(shape), None
+    else:
+        y = x.new_empty(shape, dtype=torch.float8_e4m3fn)
         scales = x.new_empty((*shape[:-1], -(-c // e4m3) if e4m3 else 1), dtype=torch.float32)
-    if y.numel():
+    n = y.numel() // c
+    if n:
         x, xs = _rows(x, c)
         rcode, rs, rp, sp = code, c, None, None
         if residual is not None:
             residual, rs = _rows(residual, c)
             rcode, rp, sp = _TOKEN_DTYPES[residual.dtype], residual.data_ptr(), summed.data_ptr()
-        weight = weight.contiguous()
-        wcode, n, st = _TOKEN_DTYPES[weight.dtype], y.numel() // c, _raw_stream(dev.index)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
         lib = _lib.load()
         if e4m3 is None:
-            _lib.check(lib.sm_rms_norm(x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), sp, code, rcode,
-                                       wcode, n, c, xs, rs, eps, st), "sm_rms_norm")
+            rc = lib.sm_rms_norm(x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), sp, code, rcode,
+                                 _TOKEN_DTYPES[weight.dtype], n, c, xs, rs, eps, _raw_stream(index))
         else:
-            _lib.check(lib.sm_rms_norm_e4m3(
-                x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), scales.data_ptr(), sp, code, rcode, wcode,
-                n, c, xs, rs, e4m3, eps, st), "sm_rms_norm_e4m3")
+            rc = lib.sm_rms_norm_e4m3(
+                x.data_ptr(), rp, weight.data_ptr(), y.data_ptr(), scales.data_ptr(), sp, code, rcode,
+                _TOKEN_DTYPES[weight.dtype], n, c, xs, rs, e4m3, eps, _raw_stream(index))
+        if rc:
+            _lib.check(rc, "sm_rms_norm")
     return (y, summed) if e4m3 is None else (y, scales, summed)
 
 
 @_on_device
-def _norm_backward(dev, summed, weight, dy, dsummed, dtype, eps):
+def _norm_backward(index, summed, weight, dy, dsummed, dtype, eps):
     """(dx, dresidual in summed's type or None where that is dx, dweight)."""
     c = summed.shape[-1]
     dx = summed.new_empty(summed.shape, dtype=dtype)
@@ -1000,7 +1021,7 @@ def _norm_backward(dev, summed, weight, dy, dsummed, dtype, eps):
         summed.data_ptr(), weight.data_ptr(), dy.data_ptr(), zp, dx.data_ptr(),
         None if dres is None else dres.data_ptr(), dw.data_ptr(), _TOKEN_DTYPES[dtype],
         _TOKEN_DTYPES[summed.dtype], _TOKEN_DTYPES[weight.dtype], n, c, ss, ys, zs, eps,
-        ws.data_ptr() if nws else None, nws, _raw_stream(dev.index)), "sm_rms_norm_backward")
+        ws.data_ptr() if nws else None, nws, _raw_stream(index)), "sm_rms_norm_backward")
     return dx, dres, dw
 
 
@@ -1009,20 +1030,20 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, eps):
         ctx.save_for_backward(x, weight)
         ctx.eps = eps
-        return _norm_forward(x.device, x, weight, None, eps)[0]
+        return _norm_forward(x.get_device(), x, weight, None, eps)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
-        dx, _, dw = _norm_backward(x.device, x, weight, dy, None, x.dtype, ctx.eps)
+        dx, _, dw = _norm_backward(x.get_device(), x, weight, dy, None, x.dtype, ctx.eps)
         return dx, dw, None
 
 
 class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        y, summed = _norm_forward(x.device, x, weight, residual, eps)
+        y, summed = _norm_forward(x.get_device(), x, weight, residual, eps)
         ctx.save_for_backward(summed, weight)
         ctx.eps, ctx.dtype = eps, x.dtype
         ctx.set_materialize_grads(False)
@@ -1036,7 +1057,7 @@ class _AddRmsNorm(torch.autograd.Function):
             if dsummed is None:
                 return None, None, None, None
             return dsummed.to(ctx.dtype), None, dsummed, None
-        dx, dres, dw = _norm_backward(summed.device, summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
+        dx, dres, dw = _norm_backward(summed.get_device(), summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
         return dx, dw, dx if dres is None else dres, None
 
 
@@ -1053,15 +1074,15 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
         if residual is None:
             return _ops().rms_norm(x, weight, float(eps))
         return _ops().add_rms_norm(x, weight, residual, float(eps))
-    _norm_checks("rms_norm", x, weight, residual, eps)
+    index = _norm_checks("rms_norm", x, weight, residual, eps)
     eps = float(eps)
     if residual is None:
         if _grads_wanted(x, weight):
             return _RmsNorm.apply(x, weight, eps)
-        return _norm_forward(x.device, x, weight, None, eps)[0]
+        return _norm_forward(index, x, weight, None, eps)[0]
     if _grads_wanted(x, weight, residual):
         return _AddRmsNorm.apply(x, weight, residual, eps)
-    return _norm_forward(x.device, x, weight, residual, eps)
+    return _norm_forward(index, x, weight, residual, eps)
 
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
@@ -1078,8 +1099,8 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
         if residual is None:
             return _ops().rms_norm_e4m3(x, weight, float(eps), group or 0)
         return _ops().add_rms_norm_e4m3(x, weight, residual, float(eps), group or 0)
-    _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
+    index = _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
     if _grads_wanted(x, weight, residual):
         raise NotImplementedError("rms_norm_e4m3 is forward only: call it under torch.no_grad()")
-    out = _norm_forward(x.device, x, weight, residual, float(eps), group or 0)
+    out = _norm_forward(index, x, weight, residual, float(eps), group or 0)
     return out[:2] if residual is None else out

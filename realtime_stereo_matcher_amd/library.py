@@ -26,13 +26,9 @@ _state = threading.local()
 def tracing() -> bool:
     """True when a functional call should go through torch.ops.stereocv (a tracer or compiler
     is recording, and the call is not already the body of one of these ops)."""
-    if getattr(_state, "inside", False):
+    if not (torch.compiler.is_compiling() or torch.jit.is_tracing()):
         return False
-    try:
-        compiling = torch.compiler.is_compiling()
-    except AttributeError:  # older torch
-        compiling = False
-    return torch.jit.is_tracing() or compiling
+    return not getattr(_state, "inside", False)
 
 
 class _Inside:
@@ -266,9 +262,9 @@ def _attn(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
           key_lengths: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
           scale: Optional[float] = None,
           max_disparity: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor]:
-    scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
-                                                     key_lengths, key_mask)
-    return F._attention_forward(query.device, query, key, value, lengths, mask, scale, band, True)
+    index, scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
+                                                            key_lengths, key_mask)
+    return F._attention_forward(index, query, key, value, lengths, mask, scale, band, True)
 
 
 def _attn_fake(query, key, value, key_lengths=None, key_mask=None, scale=None, max_disparity=None):
@@ -296,8 +292,8 @@ def _attn_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
                    key_lengths: Optional[torch.Tensor] = None,
                    key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                    max_disparity: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
-                                                     key_lengths, key_mask)
+    index, scale, band, lengths, mask = F._attention_checks(query, key, value, scale, max_disparity,
+                                                            key_lengths, key_mask)
     if out.shape != query.shape or dout.shape != query.shape or out.dtype != query.dtype \
             or dout.dtype != query.dtype or not out.is_contiguous():
         raise RuntimeError("cross_attention_backward: out and dout must have the query's shape and "
@@ -307,7 +303,7 @@ def _attn_backward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     if tuple(lse.shape) != (query.shape[0], kv, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise RuntimeError("cross_attention_backward: lse must be the forward call's")
     F._device_check(query, out, lse, dout)
-    return F._attention_backward(query.device, query, key, value, out, lse, dout, lengths, mask, scale, band)
+    return F._attention_backward(index, query, key, value, out, lse, dout, lengths, mask, scale, band)
 
 
 def _attn_backward_fake(query, key, value, out, lse, dout, key_lengths=None, key_mask=None, scale=None,
@@ -320,7 +316,7 @@ def _rot(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, la
     with _Inside(), torch.no_grad():
         if not inverse:
             return F.rotary(x, positions, frequencies, layout, amplitude)
-        return F._rotary_run(x.device, x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
+        return F._rotary_run(x.get_device(), x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
                              amplitude, True)
 
 
@@ -386,7 +382,7 @@ def _norm_backward(summed: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor,
     F._norm_checks("rms_norm_backward", dy, weight, summed, eps)
     if dsummed is not None and (dsummed.shape != summed.shape or dsummed.dtype != summed.dtype):
         raise RuntimeError("rms_norm_backward: dsummed must have summed's shape and type")
-    dx, dres, dw = F._norm_backward(summed.device, summed, weight, dy, dsummed, dy.dtype, eps)
+    dx, dres, dw = F._norm_backward(summed.get_device(), summed, weight, dy, dsummed, dy.dtype, eps)
     return dx, dx.new_empty(0, dtype=summed.dtype) if dres is None else dres, dw
 
 
