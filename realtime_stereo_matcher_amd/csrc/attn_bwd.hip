@@ -163,7 +163,7 @@ void attn_dq(Args a) {
   const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
   const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
-    const uint64_t kp = K + (uint64_t)t * KT * kb_row, vp = V + (uint64_t)t * KT * vb_row;
+    const uint64_t kp = K + (uint64_t)keys.first(t) * kb_row, vp = V + (uint64_t)keys.first(t) * vb_row;
     if (bits == keys.kAll) {
       sk.copy(kp, dst, cwave0);
       sv.copy(vp, dst + C::kTileBytes, cwave0);
@@ -206,14 +206,14 @@ void attn_dq(Args a) {
     if (seen == 0) return;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const BandOf in(a, row0, t * KT + 32 * kb, 32);
+      const BandOf in(a, row0, keys.first(t) + 32 * kb, 32);
       const unsigned seen32 = (unsigned)(seen >> (32 * kb));
       if (!in.some || seen32 == 0) continue;
       f32x16 s = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
       f32x16 ds[N];  // and the weights
       ds[0] = mma_rows<T, DP>(from, kBuf + C::kTileBytes, 32 * kb, g);
       if (!in.all || seen32 != ~0u)
-        mask_block(s, a.band > 0 ? band_bits(seen32, token - (t * KT + 32 * kb), a.band) : seen32, half);
+        mask_block(s, a.band > 0 ? band_bits(seen32, token - (keys.first(t) + 32 * kb), a.band) : seen32, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));

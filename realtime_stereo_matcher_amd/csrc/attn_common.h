@@ -332,6 +332,13 @@ __device__ __forceinline__ void load_rows(RowOps<T, DP>& f, const T* row, bool t
   }
 }
 
+// the next N instructions of the kinds in MASK, for the compiler's schedule (left to itself it reads
+// each operand just before its product and waits for LDS every time)
+constexpr int kMatrix = 0x008, kLdsRead = 0x100;
+template <int MASK, int N> __device__ __forceinline__ void order() {
+  __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
+}
+
 // the tile's rows row0 .. row0+31 times the lanes' columns
 template <typename T, int DP>
 __device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, int row0,
@@ -341,6 +348,13 @@ __device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, i
   for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
   for (int c = 0; c < Tile<T, DP>::kSteps; ++c) s = Mma<T>::mma(from.rows(tile, row0, c), f[c], s);
+  constexpr int kSteps = Tile<T, DP>::kSteps, kEarly = kSteps < 4 ? kSteps : 4;
+  order<kLdsRead, kEarly>();
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) {
+    order<kMatrix, sizeof(T) == 4 ? 4 : 1>();
+    if (c + kEarly < kSteps) order<kLdsRead, 1>();
+  }
   return s;
 }
 
@@ -376,29 +390,31 @@ struct BandOf {
   }
 };
 
-// The key tiles of a row tile: which there are, and which keys of each count.
+// The key tiles of a row tile: which there are, and which keys of each count.  The first begins at the
+// first key inside the band of the row tile's first row, so that the waves' bands cover few tiles.
 template <int KT, bool KMASK> struct Keys {
   static constexpr uint64_t kAll = KT == 64 ? ~0ull : 0xffffffffull;
   const uint8_t* mask;
-  int keys, tb, te;
+  int keys, lo, tb, te;
   __device__ __forceinline__ Keys(const Args& a, int b, int first_row, int tile_rows)
       : mask(KMASK ? a.mask + (int64_t)b * a.Lk : nullptr),
         keys(a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk) {
-    int lo = 0, hi = keys;
-    if (a.band > 0) {  // the tiles inside the band of some row
+    int hi = keys;
+    lo = tb = 0;
+    if (a.band > 0) {  // the keys inside the band of some row
       const int last = min(first_row + tile_rows, a.rows) - 1;
       lo = max(0, a.by_group(first_row) - a.band + 1);
       hi = min(keys, a.by_group(last) + 1);
     }
-    tb = lo / KT;
-    te = hi > lo ? (hi + KT - 1) / KT : tb;
+    te = hi > lo ? (hi - lo + KT - 1) / KT : 0;
   }
+  __device__ __forceinline__ int first(int t) const { return lo + t * KT; }
   __device__ __forceinline__ int byte(int t, int lane) const {
-    const int j = t * KT + lane;
+    const int j = first(t) + lane;
     return lane < KT && t < te && j < keys ? mask[j] : 0;
   }
   __device__ __forceinline__ uint64_t by_length(int t) const {
-    const int n = keys - t * KT;
+    const int n = keys - first(t);
     return n >= KT ? kAll : n <= 0 ? 0ull : (1ull << n) - 1;
   }
 };

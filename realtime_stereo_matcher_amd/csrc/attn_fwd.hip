@@ -85,7 +85,7 @@ void attn_fwd(Args a) {
   const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
   const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
-    const uint64_t kp = K + (uint64_t)t * KT * kb_row, vp = V + (uint64_t)t * KT * vb_row;
+    const uint64_t kp = K + (uint64_t)keys.first(t) * kb_row, vp = V + (uint64_t)keys.first(t) * vb_row;
     if (bits == keys.kAll) {
       sk.copy(kp, dst, cwave0);
       sv.copy(vp, dst + C::kTileBytes, cwave0);
@@ -125,7 +125,7 @@ void attn_fwd(Args a) {
     const uint64_t seen = bits;
     bits = next;
     if (seen == 0) return;  // (also a group's turn past the last tile)
-    const BandOf in(a, row0, t * KT, KT);
+    const BandOf in(a, row0, keys.first(t), KT);
     if (!in.some) return;
     f32x16 s[KB];
 #pragma unroll
@@ -134,7 +134,7 @@ void attn_fwd(Args a) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         unsigned w = (unsigned)(seen >> (32 * kb));
-        if (a.band > 0) w = band_bits(w, token - (t * KT + 32 * kb), a.band);
+        if (a.band > 0) w = band_bits(w, token - (keys.first(t) + 32 * kb), a.band);
         mask_block(s[kb], w, half);
       }
     float mx = s[0][0];
