@@ -366,6 +366,8 @@ int check_problem(const char* what, int dtype, int64_t B, int64_t Lq, int64_t Lk
   if (Lk >= (1 << 30) || (KV > 0 && Lq >= (1 << 30) / std::max<int64_t>(1, H / KV)))
     return fail(SM_EINVAL, w + ": more than 2^30 rows or keys");
   if (B >= (1 << 30) || H >= (1 << 20)) return fail(SM_EINVAL, w + ": too many batches or heads");
+  if ((double)B * (double)std::max(Lq * H, Lk * KV) * (double)D > 4e18)
+    return fail(SM_EINVAL, w + ": tensors too large");
   if (!(scale > 0.f) || scale > 3.4e38f) return fail(SM_EINVAL, w + ": the scale must be positive and finite");
   if (band < 0 || band >= (1ll << 30)) return fail(SM_EINVAL, w + ": the band must be 0 (none) to 2^30 - 1");
   return SM_OK;

@@ -233,6 +233,8 @@ def test_abi_refuses():
                     16, None, None, None, None, 0.25, 0, None, None, ws, nws, None)
 
     n = _lib.load().sm_cross_attention_backward_workspace_bytes(1, 4, 4, 2)
+    rc, msg = fwd(B=1 << 29, Lq=1 << 29, H=1 << 19, KV=1 << 19)
+    assert rc == _lib.SM_EINVAL and "too large" in msg
     for args, word in [((None, 0), "workspace"), ((P, n - 1), "workspace"), ((P + 4, n), "aligned"),
                        ((P, n, None), "null"), ((P, n, P + 2), "aligned"), ((P, n, P, P + 8), "aligned")]:
         rc, msg = bwd(*args)
@@ -288,6 +290,17 @@ ATTENTION = [
     (3, 2, 700, 4, 4, 32, None, "both"),
     (1, 40, 2500, 1, 1, 64, None, "mask"),     # ordinary rows, split keys
     (1, 20, 30, 2, 1, 32, 7, "both"),          # few rows in a band
+    # launches of 65 to 256 workgroups of 128 rows or keys: eight waves each
+    (20, 130, 140, 4, 4, 64, None, "both"),
+    (20, 130, 300, 4, 2, 32, 48, "lengths"),
+    (17, 200, 150, 4, 4, 128, None, "mask"),
+    (30, 50, 140, 9, 3, 40, None, "lengths"),  # three heads share keys: tiles begin inside a token
+    # more than 256: four waves each
+    (70, 130, 150, 4, 4, 64, None, "both"),
+    (70, 140, 150, 4, 4, 32, 24, "lengths"),
+    (70, 130, 135, 4, 4, 128, 30, "mask"),
+    (100, 50, 140, 6, 2, 40, 20, "both"),
+    (90, 129, 65, 3, 3, 16, None, None),
 ]
 
 
