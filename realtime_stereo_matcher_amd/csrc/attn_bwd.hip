@@ -76,6 +76,18 @@ __device__ __forceinline__ void join_columns(unsigned lds, int wave, int lane, i
   }
 }
 
+// A wave's products go before the other waves' vector work where the loop is long enough for the
+// waves to drift apart (4080 x 4080 tokens, 16 heads: D=64 287 -> 276 us, D=32 198 -> 184; rows of 240,
+// four tiles: 127 -> 131, and wide heads, one wave a SIMD: 655 -> 664, so not there).
+constexpr int kLongLoop = 8;
+template <int DP> __device__ __forceinline__ void products_first(bool long_loop, bool on) {
+  if constexpr (DP <= 64)
+    if (long_loop) {
+      if (on) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    }
+}
+
 // the power of two that brings x into [1/2, 1), as an exponent; 0 for 0, infinities and NaN
 __device__ __forceinline__ int down(float x) {
   const int e = (int)((__float_as_uint(x) >> 23) & 255);
@@ -184,6 +196,7 @@ void attn_dq(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
 
+  const bool long_loop = keys.te - keys.tb >= kLongLoop;
   int t = keys.tb + part;
   uint64_t bits = 0;
   int byte = 0;
@@ -223,7 +236,9 @@ void attn_dq(Args a) {
         }
         ds[0][r] = p * (ds[0][r] - delta);
       }
+      products_first<DP>(long_loop, true);
       mma_transposed<T, DP, N>(dq, from, kBuf, 32 * kb, ds);
+      products_first<DP>(long_loop, false);
     }
   };
   // every wave passes the same number of barriers: the parts' first tiles decide
@@ -364,6 +379,7 @@ void attn_dkv(Args a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
 
+  const bool long_loop = te - tb >= kLongLoop;
   int t = tb + part;
   if (t < te) copy(t, lds);
   auto step = [&](auto buf) __attribute__((always_inline)) {
@@ -410,8 +426,10 @@ void attn_dkv(Args a) {
           ds[r] = x;
         }
       }
+      products_first<DP>(long_loop, true);
       mma_transposed<T, DP>(dv, from, kAt + C::kTileBytes, 32 * rb, p);
       mma_transposed<T, DP>(dk, from, kAt, 32 * rb, ds);
+      products_first<DP>(long_loop, false);
     }
   };
   const int end = C::kAlone ? te : te + part;
