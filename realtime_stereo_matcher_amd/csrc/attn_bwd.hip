@@ -77,11 +77,11 @@ __device__ __forceinline__ void join_columns(unsigned lds, int wave, int lane, i
 }
 
 // A wave's products go before the other waves' vector work where the loop is long enough for the
-// waves to drift apart (4080 x 4080 tokens, 16 heads: D=64 287 -> 276 us, D=32 198 -> 184; rows of 240,
-// four tiles: 127 -> 131, and wide heads, one wave a SIMD: 655 -> 664, so not there).
+// waves to drift apart (4080 x 4080 tokens, 16 heads, D=64: 287 -> 276 us; wide heads, one wave a SIMD:
+// 655 -> 664; D=32 198 -> 184, but its usual rows of 240, four tiles: 127 -> 131).
 constexpr int kLongLoop = 8;
 template <int DP> __device__ __forceinline__ void products_first(bool long_loop, bool on) {
-  if constexpr (DP <= 64)
+  if constexpr (DP == 64)
     if (long_loop) {
       if (on) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(0);

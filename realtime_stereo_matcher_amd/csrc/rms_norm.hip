@@ -161,7 +161,7 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void forward(Args a) {
       float w[8];
       get8_of<T>(w, a.w, c, a.w_type, n, a.vec & kVecW);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * inv * w[e];
+      for (int e = 0; e < 8; ++e) v[k][e] = Q8 ? v[k][e] * w[e] : v[k][e] * inv * w[e];
       if constexpr (!Q8)
         put8(static_cast<T*>(a.y) + row * a.C + c, v[k], n, a.vec & kVecY);
       else
@@ -187,14 +187,19 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void forward(Args a) {
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + t) * 8, n = there ? a.C - c : 0;
       if (n <= 0) continue;
-      const float scale = top[k] == 0.f ? 1.f : top[k] / 448.f;
+      // y / scale = s w 448 / max |s w|: the root cancels, and one rounding less than y and scale
+      // would carry lands on a border between two codes less often
+      const float most = top[k], y_most = most * inv;
+      const float scale = y_most == 0.f ? 1.f : y_most / 448.f;
+      const float by = 448.f / most;
+      const bool tame = most > 0x1p-100f && most < 0x1p100f;
       const int g = a.groups == 1 ? 0 : c / 128;
       if (a.groups == 1 ? c == 0 : c % 128 == 0) a.scale[row * a.groups + g] = scale;
       unsigned p[2];
       float z[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {  // NaN stays NaN
-        z[e] = v[k][e] / scale;
+        z[e] = y_most == 0.f ? 0.f : tame ? v[k][e] * by : v[k][e] / most * 448.f;
         z[e] = z[e] > 448.f ? 448.f : z[e] < -448.f ? -448.f : z[e];
       }
 #pragma unroll
@@ -223,13 +228,17 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void backward(Args a) {
   __shared__ float join[kRowsWg > 1 ? kThreads * 8 : 1];
   int slot = 0;
   const int t = threadIdx.x % TPR;
-  float dw[NV][8], w[NV][8];
+  constexpr bool kKeep = TPR <= 256;  // the weights in registers (1024 threads have 128 each)
+  float dw[NV][8], w[kKeep ? NV : 1][8];
+  auto weights = [&](int k) {
+    const int c = (k * TPR + t) * 8;
+    if (c < a.C) get8_of<T>(w[kKeep ? k : 0], a.w, c, a.w_type, a.C - c, a.vec & kVecW);
+  };
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = (k * TPR + t) * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[k][e] = w[k][e] = 0.f;
-    if (c < a.C) get8_of<T>(w[k], a.w, c, a.w_type, a.C - c, a.vec & kVecW);
+    for (int e = 0; e < 8; ++e) dw[k][e] = w[kKeep ? k : 0][e] = 0.f;
+    if (kKeep) weights(k);
   }
   const int64_t sets = (a.rows + kRowsWg - 1) / kRowsWg;
   for (int64_t set = blockIdx.x; set < sets; set += gridDim.x) {
@@ -244,10 +253,11 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void backward(Args a) {
       if (n > 0) {
         get8_of<T>(s[k], a.s, row * a.xs + c, a.r_type, n, a.vec & kVecS);
         get8(h[k], static_cast<const T*>(a.dy) + row * a.ys + c, n, a.vec & kVecY);
+        if (!kKeep) weights(k);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           sums[0] = fmaf(s[k][e], s[k][e], sums[0]);
-          sums[1] = fmaf(h[k][e] * w[k][e], s[k][e], sums[1]);
+          sums[1] = fmaf(h[k][e] * w[kKeep ? k : 0][e], s[k][e], sums[1]);
         }
       }
     }
@@ -262,10 +272,11 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void backward(Args a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = 0.f;
       if (a.ds != nullptr) get8_of<T>(z, a.ds, row * a.zs + c, a.r_type, n, a.vec & kVecZ);
+      if (!kKeep) weights(k);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         dw[k][e] = fmaf(h[k][e] * inv, s[k][e], dw[k][e]);
-        z[e] += h[k][e] * w[k][e] * inv - s[k][e] * back;
+        z[e] += h[k][e] * w[kKeep ? k : 0][e] * inv - s[k][e] * back;
       }
       put8(static_cast<T*>(a.dx) + row * a.C + c, z, n, a.vec & kVecD);
       if (a.dr != nullptr) put8(static_cast<float*>(a.dr) + row * a.C + c, z, n, a.vec & kVecDr);

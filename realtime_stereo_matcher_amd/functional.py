@@ -658,6 +658,15 @@ def _token_ready(t, group=1):
     return t.clone(memory_format=torch.contiguous_format), None
 
 
+def _first_order(fn):
+    """once_differentiable, without its cost where no second derivative can follow."""
+    with_graph = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return with_graph(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return backward
+
+
 def _grads_wanted(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -718,7 +727,7 @@ class _CrossAttention(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout, _):
         q, k, v, out, lse, lengths, mask = ctx.saved_tensors
         return (*_attention_backward(q.get_device(), q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.band),
@@ -884,7 +893,7 @@ class _Rotary(torch.autograd.Function):
         return _rotary_run(x.get_device(), x, positions, frequencies, interleaved, amplitude, False)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         return (_rotary_run(dy.get_device(), dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
 
@@ -1033,7 +1042,7 @@ class _RmsNorm(torch.autograd.Function):
         return _norm_forward(x.get_device(), x, weight, None, eps)[0]
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         dx, _, dw = _norm_backward(x.get_device(), x, weight, dy, None, x.dtype, ctx.eps)
@@ -1050,7 +1059,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return y, summed
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dsummed):
         summed, weight = ctx.saved_tensors
         if dy is None:  # only the stream was used
