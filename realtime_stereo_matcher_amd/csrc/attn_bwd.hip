@@ -116,6 +116,7 @@ void attn_dq(Args a) {
   const bool there = row < a.rows;
 
   Keys<KT, KMASK> keys(a, b, wg_row0, C::kTileRows);
+  if (wg_row0 >= a.rows) keys.te = keys.tb;  // padding: its lse and delta alone
 
   const int64_t orow = (((int64_t)b * a.Lq + token) * a.H + head) * a.D;
   RowOps<T, DP> q, g;
@@ -218,7 +219,7 @@ void attn_dq(Args a) {
     }
     const uint64_t seen = bits;
     bits = next;
-    if (seen == 0) return;
+    if (seen == 0 || row0 >= a.rows) return;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const BandOf in(a, row0, keys.first(t) + 32 * kb, 32);

@@ -131,7 +131,8 @@ void attn_fwd(Args a) {
     }
     const uint64_t seen = bits;
     bits = next;
-    if (seen == 0) return;  // (also a group's turn past the last tile)
+    // (also a group's turn past the last tile, and a wave whose rows lie past the end)
+    if (seen == 0 || row0 >= a.rows) return;
     const BandOf in(a, row0, keys.first(t), KT);
     if (!in.some) return;
     f32x16 s[KB];
