@@ -433,12 +433,11 @@ template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 v) {
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<f32x4*>(p) = v;
   } else {
-    T t[4];
+    Frag<T> f = {};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = from_f<T>(v[e]);
-    u32x2 u;
-    __builtin_memcpy(&u, t, 8);
-    *reinterpret_cast<u32x2*>(p) = u;
+    for (int e = 0; e < 4; ++e) Mma<T>::put(f, e, v[e]);
+    const u32x4 u = __builtin_bit_cast(u32x4, f);
+    *reinterpret_cast<u32x2*>(p) = u32x2{u[0], u[1]};
   }
 }
 
