@@ -47,7 +47,9 @@ template <typename T, int DP, int MODE> struct BCfg {
   static constexpr int kBufQ = 2 * kTileBytes;         // keys and values
   static constexpr int kBufKv = 2 * kTileBytes + 512;  // rows, gradients, lse and delta
   static constexpr int kJoin = kParts > 1 ? kWaves * 32 * (DP + 4) * 4 : 0;
-  static constexpr int kLdsQ = kJoin > 2 * kBufQ * kParts ? kJoin : 2 * kBufQ * kParts;
+  static constexpr int kTilesQ = 2 * kBufQ * kParts;
+  static constexpr int kMaskQ = 2 * kTile * 4 * kParts;  // 0 or -inf for each key of a buffer
+  static constexpr int kLdsQ = kJoin > kTilesQ + kMaskQ ? kJoin : kTilesQ + kMaskQ;
   static constexpr int kLdsKv = kJoin > 2 * kBufKv * kParts ? kJoin : 2 * kBufKv * kParts;
   // waves a SIMD: two where the accumulators leave room for them
   static constexpr int kResident = kAlone || DP == 128 || (kWide && DP == 64) ? 1 : 2;
@@ -177,6 +179,11 @@ void attn_dq(Args a) {
   sv.init(ctid, a.D, [&](int r) { return r * vb_row; });
   const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
   const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
+  const unsigned minus_inf = lds_addr(smem) + C::kTilesQ + part * 2 * KT * 4;
+  auto put_mask = [&](int buf, uint64_t bits) {
+    if (KMASK && cwave0 == 0 && lane < KT)
+      lds_put(minus_inf + buf * KT * 4 + lane * 4, (bits >> lane) & 1 ? 0.f : -INFINITY);
+  };
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
     const uint64_t kp = K + (uint64_t)keys.first(t) * kb_row, vp = V + (uint64_t)keys.first(t) * vb_row;
     if (bits == keys.kAll) {
@@ -206,6 +213,7 @@ void attn_dq(Args a) {
   if (t < keys.te) {
     bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
     copy(t, lds, bits);
+    put_mask(0, bits);
   }
   if (KMASK) byte = keys.byte(t + C::kParts, lane);
   auto step = [&](auto buf) __attribute__((always_inline)) {
@@ -216,6 +224,7 @@ void attn_dq(Args a) {
       next = KMASK ? __ballot(byte) : keys.by_length(t + C::kParts);
       if (KMASK) byte = keys.byte(t + 2 * C::kParts, lane);
       copy(t + C::kParts, lds + (C::kBufQ - kBuf), next);
+      put_mask(1 - decltype(buf)::value, next);
     }
     const uint64_t seen = bits;
     bits = next;
@@ -225,11 +234,17 @@ void attn_dq(Args a) {
       const BandOf in(a, row0, keys.first(t) + 32 * kb, 32);
       const unsigned seen32 = (unsigned)(seen >> (32 * kb));
       if (!in.some || seen32 == 0) continue;
-      f32x16 s = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
+      f32x16 s;
+      if constexpr (KMASK)
+        s = mma_rows_masked<T, DP>(minus_inf + (decltype(buf)::value * KT + 32 * kb + 4 * half) * 4, from,
+                                   kBuf, 32 * kb, q);
+      else
+        s = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
       f32x16 ds[N];  // and the weights
       ds[0] = mma_rows<T, DP>(from, kBuf + C::kTileBytes, 32 * kb, g);
-      if (!in.all || seen32 != ~0u)
-        mask_block(s, a.band > 0 ? band_bits(seen32, token - (keys.first(t) + 32 * kb), a.band) : seen32, half);
+      const unsigned left = KMASK ? ~0u : seen32;
+      if (!in.all || left != ~0u)
+        mask_block(s, a.band > 0 ? band_bits(left, token - (keys.first(t) + 32 * kb), a.band) : left, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));

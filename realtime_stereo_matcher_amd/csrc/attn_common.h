@@ -339,23 +339,45 @@ template <int MASK, int N> __device__ __forceinline__ void order() {
   __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
 }
 
-// the tile's rows row0 .. row0+31 times the lanes' columns
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, int row0,
-                                           const RowOps<T, DP>& f) {
-  f32x16 s;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+// the tile's rows row0 .. row0+31 times the lanes' columns, added to `s` (which READS LDS reads form)
+template <typename T, int DP, int READS>
+__device__ __forceinline__ f32x16 mma_rows_to(f32x16 s, const Reads<T, DP>& from, int tile, int row0,
+                                              const RowOps<T, DP>& f) {
 #pragma unroll
   for (int c = 0; c < Tile<T, DP>::kSteps; ++c) s = Mma<T>::mma(from.rows(tile, row0, c), f[c], s);
   constexpr int kSteps = Tile<T, DP>::kSteps, kEarly = kSteps < 4 ? kSteps : 4;
-  order<kLdsRead, kEarly>();
+  order<kLdsRead, kEarly + READS>();
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) {
     order<kMatrix, sizeof(T) == 4 ? 4 : 1>();
     if (c + kEarly < kSteps) order<kLdsRead, 1>();
   }
   return s;
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 mma_rows(const Reads<T, DP>& from, int tile, int row0,
+                                           const RowOps<T, DP>& f) {
+  f32x16 zero;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+  return mma_rows_to<T, DP, 0>(zero, from, tile, row0, f);
+}
+// The same for masked keys, from 0 for a key that counts and -inf for another: rows of `at`, from the
+// lane's half on.  A masked row of the tile holds a finite copy of another, so its score is -inf without
+// vector work (2 x 1021 x 4093 tokens, 16 heads over 4, D=64, bf16, with holes: forward 71 -> 61 us against
+// two bit operations a score; 540 x 960 x 960, 2 heads of 32, fp16: backward 772 -> 727 us).
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 mma_rows_masked(unsigned at, const Reads<T, DP>& from, int tile, int row0,
+                                                  const RowOps<T, DP>& f) {
+  f32x16 s;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 x = lds_get<f32x4>(at + 32 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[4 * g + e] = x[e];
+  }
+  return mma_rows_to<T, DP, 4>(s, from, tile, row0, f);
 }
 
 // The keys of a 32-key block that the lane's token may see, bit j for key j: those that exist and are

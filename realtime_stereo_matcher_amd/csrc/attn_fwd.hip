@@ -9,7 +9,7 @@
 //
 // Bound by the matrix unit for wide heads (8160 x 8100 tokens, 16 heads, D=128, bf16: 530 us, 1020
 // TFLOP/s; 455 us without any softmax work, which is what large library products reach too), by the
-// exponentials and the other vector work for narrow ones (D=32: 220 us), by HBM for single tokens (four
+// exponentials and the other vector work for narrow ones (D=32: 212 us), by HBM for single tokens (four
 // of 8 to 16 thousand keys, 8 key heads, D=128: 201 MB in 45 us).  Four waves of 32 rows: 64-row
 // workgroups copy the keys too often (854 us at D=128), 256-row ones wait for each other (553 us, and
 // 115 us instead of 92 for 540 rows of 960 in a band of 192).
@@ -38,8 +38,9 @@ template <typename T, int DP, bool FEW, int GROUPS> struct Cfg {
   static constexpr int kBufBytes = 2 * kTileBytes;  // keys and values
   // two buffers a part; the join needs a wave's sums and statistics each
   static constexpr int kTiles = 2 * kBufBytes * kParts;
+  static constexpr int kMask = 2 * kTile * 4 * kParts;  // 0 or -inf for each key of a buffer
   static constexpr int kJoin = kParts > 1 ? kWaves * (32 * (DP + 4) * 4 + 256) : 0;
-  static constexpr int kLds = kTiles > kJoin ? kTiles : kJoin;
+  static constexpr int kLds = kTiles + kMask > kJoin ? kTiles + kMask : kJoin;
 };
 
 constexpr float kLazy = 8.f;
@@ -91,6 +92,11 @@ void attn_fwd(Args a) {
   sv.init(ctid, a.D, [&](int r) { return r * vb_row; });
   const uint64_t K = reinterpret_cast<uint64_t>(static_cast<const T*>(a.k) + b * a.ks[0] + kv * a.ks[2]);
   const uint64_t V = reinterpret_cast<uint64_t>(static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2]);
+  const unsigned minus_inf = lds_addr(smem) + C::kTiles + part * 2 * KT * 4;
+  auto put_mask = [&](int buf, uint64_t bits) {
+    if (KMASK && cwave0 == 0 && lane < KT)
+      lds_put(minus_inf + buf * KT * 4 + lane * 4, (bits >> lane) & 1 ? 0.f : -INFINITY);
+  };
   auto copy = [&](int t, unsigned dst, uint64_t bits) {
     const uint64_t kp = K + (uint64_t)keys.first(t) * kb_row, vp = V + (uint64_t)keys.first(t) * vb_row;
     if (bits == keys.kAll) {
@@ -116,6 +122,7 @@ void attn_fwd(Args a) {
   if (t < keys.te) {
     bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
     copy(t, lds, bits);
+    put_mask(0, bits);
   }
   if (KMASK) byte = keys.byte(t + kStep, lane);
 
@@ -128,6 +135,7 @@ void attn_fwd(Args a) {
       next = KMASK ? __ballot(byte) : keys.by_length(t + kStep);
       if (KMASK) byte = keys.byte(t + 2 * kStep, lane);
       copy(t + kStep, lds + (C::kBufBytes - kBuf), next);
+      put_mask(1 - decltype(buf)::value, next);
     }
     const uint64_t seen = bits;
     bits = next;
@@ -137,11 +145,16 @@ void attn_fwd(Args a) {
     if (!in.some) return;
     f32x16 s[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
-    if (!in.all || seen != keys.kAll)
+    for (int kb = 0; kb < KB; ++kb)
+      if constexpr (KMASK)
+        s[kb] = mma_rows_masked<T, DP>(minus_inf + (decltype(buf)::value * KT + 32 * kb + 4 * half) * 4, from,
+                                       kBuf, 32 * kb, q);
+      else
+        s[kb] = mma_rows<T, DP>(from, kBuf, 32 * kb, q);
+    if (!in.all || (!KMASK && seen != keys.kAll))
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        unsigned w = (unsigned)(seen >> (32 * kb));
+        unsigned w = KMASK ? ~0u : (unsigned)(seen >> (32 * kb));
         if (a.band > 0) w = band_bits(w, token - (keys.first(t) + 32 * kb), a.band);
         mask_block(s[kb], w, half);
       }
