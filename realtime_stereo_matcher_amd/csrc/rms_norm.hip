@@ -9,7 +9,8 @@
 // both its statistics and its outputs come from there.  Sums are fp32.  A row has 4 to 1024 threads,
 // so that a wave holds whole rows of narrow maps and a workgroup one wide row.  518,400 rows of 64,
 // bf16 with residual: forward 265 MB in 46 us, backward the same in 56 us and 6 us for the sum of dw;
-// 32,760 rows of 5000, fp16 with a 32-bit stream, to e4m3: 1.8 GB in 349 us (5.2 TB/s).
+// 32,760 rows of 5000, fp16 with a 32-bit stream, to e4m3: 1.8 GB in 359 us (5.0 TB/s;
+// 350 with the codes' last two steps in 32 bits, which moved about one code in a million).
 #include <algorithm>
 #include <type_traits>
 
@@ -163,45 +164,71 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void forward(Args a) {
       float w[8];
       get8_of<T>(w, a.w, c, a.w_type, n, a.vec & kVecW);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = Q8 ? v[k][e] * w[e] : v[k][e] * inv * w[e];
-      if constexpr (!Q8)
-        put8(static_cast<T*>(a.y) + row * a.C + c, v[k], n, a.vec & kVecY);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top[k] = larger(top[k], fabsf(v[k][e]));
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (Q8) top[k] = larger(top[k], fabsf(v[k][e] * w[e]));
+        else v[k][e] = v[k][e] * inv * w[e];
+      }
+      if constexpr (!Q8) put8(static_cast<T*>(a.y) + row * a.C + c, v[k], n, a.vec & kVecY);
     }
   }
   if constexpr (Q8) {
-    if (a.groups == 1) {
+    auto over_group = [&](float (&m)[NV]) {
+      if (a.groups == 1) {
 #pragma unroll
-      for (int k = 1; k < NV; ++k) top[0] = larger(top[0], top[k]);
-      float one[1] = {top[0]};
-      over_row<TPR, true>(one, lds, slot);
+        for (int k = 1; k < NV; ++k) m[0] = larger(m[0], m[k]);
+        float one[1] = {m[0]};
+        over_row<TPR, true>(one, lds, slot);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) top[k] = one[0];
-    } else {  // 128 values are 16 neighbouring threads' of one step (narrower rows: one group)
+        for (int k = 0; k < NV; ++k) m[k] = one[0];
+      } else {  // 128 values are 16 neighbouring threads' of one step (narrower rows: one group)
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1)
+        for (int o = 1; o < 16; o <<= 1)
 #pragma unroll
-        for (int k = 0; k < NV; ++k) top[k] = larger(top[k], __shfl_xor(top[k], o));
+          for (int k = 0; k < NV; ++k) m[k] = larger(m[k], __shfl_xor(m[k], o));
+      }
+    };
+    float mine[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) mine[k] = top[k];
+    over_group(top);
+    // What the largest |s w| lost to its rounding, plus a unit (so that it is positive): of the values
+    // that round to it, the largest.  Products of two 16-bit values are exact.
+    float low[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) low[k] = 0.f;
+    if (sizeof(T) == 4 || a.r_type == kF32 || a.w_type == kF32) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * TPR + t) * 8, n = there ? a.C - c : 0;
+        if (n <= 0 || mine[k] != top[k] || !(top[k] > 0x1p-60f && top[k] < INFINITY)) continue;
+        float w[8];
+        get8_of<T>(w, a.w, c, a.w_type, n, a.vec & kVecW);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = v[k][e] * w[e], lost = fmaf(v[k][e], w[e], -p);
+          if (fabsf(p) == top[k]) low[k] = larger(low[k], top[k] * 0x1p-23f + (p < 0.f ? -lost : lost));
+        }
+      }
+      over_group(low);
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + t) * 8, n = there ? a.C - c : 0;
       if (n <= 0) continue;
-      // y / scale = s w 448 / max |s w|: the root cancels, and one rounding less than y and scale
-      // would carry lands on a border between two codes less often
+      // y / scale = s w 448 / max |s w|: the root cancels, and formed in 64 bits the value is rounded
+      // once to 32 before it is rounded to 8, so no code on a border between two is left to chance
       const float most = top[k], y_most = most * inv;
       const float scale = y_most == 0.f ? 1.f : y_most / 448.f;
-      const float by = 448.f / most;
-      const bool tame = most > 0x1p-100f && most < 0x1p100f;
+      const double by = 448.0 / (low[k] > 0.f ? (double)most + ((double)low[k] - (double)(most * 0x1p-23f)) : (double)most);
+      float w[8];
+      get8_of<T>(w, a.w, c, a.w_type, n, a.vec & kVecW);
       const int g = a.groups == 1 ? 0 : c / 128;
       if (a.groups == 1 ? c == 0 : c % 128 == 0) a.scale[row * a.groups + g] = scale;
       unsigned p[2];
       float z[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {  // NaN stays NaN
-        z[e] = y_most == 0.f ? 0.f : tame ? v[k][e] * by : v[k][e] / most * 448.f;
+        z[e] = y_most == 0.f ? 0.f : (float)((double)v[k][e] * (double)w[e] * by);
         z[e] = z[e] > 448.f ? 448.f : z[e] < -448.f ? -448.f : z[e];
       }
 #pragma unroll

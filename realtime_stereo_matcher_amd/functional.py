@@ -1098,7 +1098,7 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
     """``rms_norm`` with y in 8 bits, for a product that takes them: ``(q, scales)``, or ``(q, scales,
     s)`` with a residual, where ``y ~ q * scales``.
 
-    q is (..., C) float8_e4m3fn, rounded to nearest from the fp32 y / scale; a scale is max|y| / 448
+    q is (..., C) float8_e4m3fn, the code nearest to y / scale (formed in 64 bits); a scale is max|y| / 448
     over the row (``group=None``; scales (..., 1)) or over each 128 values of it (``group=128``; scales
     (..., ceil(C / 128))), and 1 where y is 0.  Forward only.
     """

@@ -648,6 +648,25 @@ def test_rms_norm_e4m3(rows, c, group, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=name)
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("rows,c", [(6000, 1000), (40000, 64), (700, 5000), (60, 20000)])
+def test_rms_norm_e4m3_codes(rows, c, group, dtype):
+    """s w 448 / max |s w| in 64 bits, rounded to 32 and then to 8: none of a million codes differs (the
+    kernel's 64-bit value is within 4 units of 2^-53, which decides a rounding to 32 bits once in 2^27)."""
+    for kind in kinds(dtype):
+        x, w, r, _, _ = norm_inputs(rows, c, dtype, *kind, seed=c)
+        s = x if r is None else (x.double() + r.double()).to(r.dtype)
+        sw = s.double() * w.double()
+        parts = sw.split(group or c, -1)
+        want = torch.cat([(p * (448 / p.abs().amax(-1, keepdim=True))).float().to(torch.float8_e4m3fn)
+                          for p in parts], -1)
+        q = F.rms_norm_e4m3(*cuda(x, w, r), group=group)[0].cpu()
+        differ = int((q.view(torch.uint8) != want.view(torch.uint8)).sum())
+        assert differ == 0, (kind, differ)
+
+
+@gpu
 def test_rms_norm_special_rows():
     """Rows of zeros, of one value, with NaN or infinity: they stay in their rows."""
     x = torch.ones(6, 300, device="cuda")
