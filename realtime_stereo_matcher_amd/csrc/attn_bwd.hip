@@ -11,9 +11,10 @@
 //   attn_dq   a wave owns 32 query rows; writes dq, and per row delta and the logarithm in base 2.
 //             In 16 bits g . o carries the rounding of o and of the weights that formed it, which
 //             shifts a whole row of ds.  So the row's delta = sum_j p_ij (g_i . v_j) is summed in
-//             fp32 beside the products: attn_dkv takes that one, and dq, formed with g . o, is put
-//             right at the end by the difference times sum_j p_ij k_j (one product more, on the
-//             keys already read).
+//             fp32 beside the products for attn_dkv.  dq is formed with g . o and put right at the
+//             end: exact ds sum to 0 over a row's keys, so what the rounded ones sum to, times
+//             sum_j p_ij k_j (one product more, on the keys already read), is taken off.  That is
+//             delta's error and, with it, the part of ds' own rounding that meets the keys' mean.
 //   attn_dkv  a wave owns 32 keys; loops over the rows of all heads that share them
 // fp16: ds would fall out of the type's range for small gradients, so g enters with a power of
 // two: one that brings the row's largest |g| into [1/2, 1) in attn_dq (a lane's scalar), the
@@ -198,7 +199,8 @@ void attn_dq(Args a) {
   // dq, and (16-bit types) the weighted mean of the keys
   constexpr int N = sizeof(T) == 4 ? 1 : 2;
   f32x16 dq[N][DP / 32];
-  float sum = 0.f;  // of p (g . v): delta again
+  float sum = 0.f;      // of p (g . v): delta again
+  float rounded = 0.f;  // of ds as it enters the product
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -254,6 +256,9 @@ void attn_dq(Args a) {
         }
         ds[0][r] = p * (ds[0][r] - delta);
       }
+      if constexpr (N == 2)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) rounded = Mma<T>::add2(ds[0][r], ds[0][r + 1], rounded);
       products_first<DP>(long_loop, true);
       mma_transposed<T, DP, N>(dq, from, kBuf, 32 * kb, ds);
       products_first<DP>(long_loop, false);
@@ -272,21 +277,27 @@ void attn_dq(Args a) {
   if constexpr (C::kParts > 1) __syncthreads();
   if constexpr (N == 2) {
     sum = other_half_sum(sum);
+    rounded = other_half_sum(rounded);
     if constexpr (C::kParts > 1) {
-      if (half == 0) lds_put(base + (wave * 32 + lane) * 4, sum);
+      const unsigned second = base + C::kWaves * 32 * 4;
+      if (half == 0) {
+        lds_put(base + (wave * 32 + lane) * 4, sum);
+        lds_put(second + (wave * 32 + lane) * 4, rounded);
+      }
       __syncthreads();
-      sum = 0.f;
+      sum = rounded = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::kParts; ++w)
+      for (int w = 0; w < C::kParts; ++w) {
         sum += lds_get<float>(base + ((w * C::kSets + set) * 32 + (lane & 31)) * 4);
+        rounded += lds_get<float>(second + ((w * C::kSets + set) * 32 + (lane & 31)) * 4);
+      }
       __syncthreads();
     }
     if (half == 0 && part == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift);
-    delta -= sum;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(delta, dq[1][db][r], dq[0][db][r]);
+      for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(-rounded, dq[1][db][r], dq[0][db][r]);
   }
   const float by = __builtin_ldexpf(a.scale, -shift);
   if constexpr (C::kParts > 1) {

@@ -71,6 +71,10 @@ template <> struct Mma<__half> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ void put(frag& f, int e, float v) { f[e] = (_Float16)v; }
+  static __device__ __forceinline__ float add2(float a, float b, float c) {  // rounded, summed in fp32
+    typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(h16x2{(_Float16)a, (_Float16)b}, h16x2{1, 1}, c, false);
+  }
   static __device__ __forceinline__ float get(const frag& f, int e) { return (float)f[e]; }
 };
 template <> struct Mma<bf16_t> {
@@ -79,6 +83,10 @@ template <> struct Mma<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ void put(frag& f, int e, float v) { f[e] = (__bf16)v; }
+  static __device__ __forceinline__ float add2(float a, float b, float c) {
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(b16x2{(__bf16)a, (__bf16)b}, b16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+  }
   static __device__ __forceinline__ float get(const frag& f, int e) { return (float)f[e]; }
 };
 // fp32: four 32x32x2 steps a 16-byte piece; step e contracts values 8c + e and 8c + 4 + e.
