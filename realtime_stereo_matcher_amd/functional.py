@@ -885,31 +885,9 @@ def _rotary_run(index, x, positions, frequencies, interleaved, amplitude, invers
     return y
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, frequencies, interleaved, amplitude):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.how = interleaved, amplitude
-        return _rotary_run(x.get_device(), x, positions, frequencies, interleaved, amplitude, False)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, dy):
-        return (_rotary_run(dy.get_device(), dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
-
-
-def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
-    """Rotary positions of (B,L,heads,D) tokens: the first ``2 * len(frequencies)`` values of every
-    head are turned in pairs by ``positions * frequencies`` radians, the others pass through.
-
-    ``positions``: (L,) or (B,L) int32 / int64; ``frequencies``: float64 on the tokens' device, kept by
-    the caller (``rotary_frequencies``).  ``layout``: ``"half"`` pairs value n with n + R/2,
-    ``"interleaved"`` 2n with 2n + 1.  ``amplitude`` multiplies the turned values.  The angle is formed
-    in 64 bits, so far positions are as exact as near ones; one rounding, to the tokens' type.
-    Differentiable in x.
-    """
-    if _traced():
-        return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
+def _rotary_checks(x, positions, frequencies, layout):
+    """(device index, positions, frequencies) as the kernel takes them, or the refusal: for the turn and
+    the turn back."""
     what = "rotary"
     _tensors(what, "x", x, "positions", positions, "frequencies", frequencies)
     shape, pshape = x.shape, positions.shape
@@ -935,6 +913,35 @@ def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
         positions = positions.contiguous()
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
+    return index, positions, frequencies
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, interleaved, amplitude):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = interleaved, amplitude
+        return _rotary_run(x.get_device(), x, positions, frequencies, interleaved, amplitude, False)
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, dy):
+        return (_rotary_run(dy.get_device(), dy, *ctx.saved_tensors, *ctx.how, True), None, None, None, None)
+
+
+def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
+    """Rotary positions of (B,L,heads,D) tokens: the first ``2 * len(frequencies)`` values of every
+    head are turned in pairs by ``positions * frequencies`` radians, the others pass through.
+
+    ``positions``: (L,) or (B,L) int32 / int64; ``frequencies``: float64 on the tokens' device, kept by
+    the caller (``rotary_frequencies``).  ``layout``: ``"half"`` pairs value n with n + R/2,
+    ``"interleaved"`` 2n with 2n + 1.  ``amplitude`` multiplies the turned values.  The angle is formed
+    in 64 bits, so far positions are as exact as near ones; one rounding, to the tokens' type.
+    Differentiable in x.
+    """
+    if _traced():
+        return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
+    index, positions, frequencies = _rotary_checks(x, positions, frequencies, layout)
     interleaved, amplitude = layout == "interleaved", float(amplitude)
     if x.requires_grad and torch.is_grad_enabled():
         return _Rotary.apply(x, positions, frequencies, interleaved, amplitude)

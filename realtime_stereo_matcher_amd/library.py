@@ -313,11 +313,8 @@ def _attn_backward_fake(query, key, value, out, lse, dout, key_lengths=None, key
 
 def _rot(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half",
          amplitude: float = 1.0, inverse: bool = False) -> torch.Tensor:
-    with _Inside(), torch.no_grad():
-        if not inverse:
-            return F.rotary(x, positions, frequencies, layout, amplitude)
-        return F._rotary_run(x.get_device(), x, positions.contiguous(), frequencies.contiguous(), layout == "interleaved",
-                             amplitude, True)
+    index, positions, frequencies = F._rotary_checks(x, positions, frequencies, layout)
+    return F._rotary_run(index, x, positions, frequencies, layout == "interleaved", amplitude, inverse)
 
 
 def _rot_fake(x, positions, frequencies, layout="half", amplitude=1.0, inverse=False):
