@@ -376,10 +376,12 @@ def _add_norm_grad(ctx, dy, dsummed):
 def _norm_backward(summed: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor,
                    dsummed: Optional[torch.Tensor] = None,
                    eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    F._norm_checks("rms_norm_backward", dy, weight, summed, eps)
-    if dsummed is not None and (dsummed.shape != summed.shape or dsummed.dtype != summed.dtype):
-        raise RuntimeError("rms_norm_backward: dsummed must have summed's shape and type")
-    dx, dres, dw = F._norm_backward(summed.get_device(), summed, weight, dy, dsummed, dy.dtype, eps)
+    index = F._norm_checks("rms_norm_backward", dy, weight, summed, eps)
+    if dsummed is not None:
+        if dsummed.shape != summed.shape or dsummed.dtype != summed.dtype:
+            raise RuntimeError("rms_norm_backward: dsummed must have summed's shape and type")
+        F._one_device(summed, dsummed)
+    dx, dres, dw = F._norm_backward(index, summed, weight, dy, dsummed, dy.dtype, eps)
     return dx, dx.new_empty(0, dtype=summed.dtype) if dres is None else dres, dw
 
 

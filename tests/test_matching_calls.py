@@ -72,3 +72,55 @@ def test_rotary_op_refuses(case, inverse, request):
     call = library._rot if case == "device" else ops.rotary  # (a meta tensor would select the fake kernel)
     with pytest.raises(error):
         call(x, p, f, layout, 1.0, inverse)
+
+
+@pytest.mark.parametrize("case", ["fine", "shape", "type", "device", "weight", "summed shape", "summed type", "host"])
+def test_norm_backward_op_refuses(case, request):
+    """Every tensor of the gradients' call is checked, the stream's gradient among them."""
+    if case != "host":
+        request.getfixturevalue("no_launch")
+    s, w, dy, ds, error = torch.zeros(3, 8), torch.zeros(8), torch.zeros(3, 8).half(), torch.zeros(3, 8), RuntimeError
+    if case == "fine":
+        error = Reached
+    elif case == "shape":
+        ds = ds[:2]
+    elif case == "type":
+        ds = ds.half()
+    elif case == "device":
+        ds = ds.to("meta")
+    elif case == "weight":
+        w = w[:7]
+    elif case == "summed shape":
+        s, ds = s[:2], ds[:2]
+    elif case == "summed type":
+        s, ds, error = s.bfloat16(), ds.bfloat16(), TypeError
+    call = library._norm_backward if case == "device" else ops.rms_norm_backward
+    with pytest.raises(error):
+        call(s, w, dy, ds, 1e-6)
+
+
+@pytest.mark.parametrize("case", ["fine", "out", "dout type", "lse", "lse type", "device", "dout device", "mask", "host"])
+def test_attention_backward_op_refuses(case, request):
+    if case != "host":
+        request.getfixturevalue("no_launch")
+    q, k, lse, error = torch.zeros(2, 5, 4, 16), torch.zeros(2, 7, 2, 16), torch.zeros(2, 2, 10), RuntimeError
+    out, dout, mask = q.clone(), q.clone(), None
+    if case == "fine":
+        error = Reached
+    elif case == "out":
+        out = out[:, :4]
+    elif case == "dout type":
+        dout = dout.half()
+    elif case == "lse":
+        lse = lse[:, :, :9]
+    elif case == "lse type":
+        lse = lse.double()
+    elif case == "device":
+        lse = lse.to("meta")
+    elif case == "dout device":
+        dout = dout.to("meta")
+    elif case == "mask":
+        mask = torch.ones(2, 6, dtype=torch.bool)
+    call = library._attn_backward if "device" in case else ops.cross_attention_backward
+    with pytest.raises(error):
+        call(q, k, k, out, lse, dout, None, mask)
