@@ -31,6 +31,7 @@ import numpy as np
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -658,11 +659,20 @@ def _token_ready(t, group=1):
     return t.clone(memory_format=torch.contiguous_format), None
 
 
+def _no_tangents(what, *ts):
+    """Refuse tensors with a tangent: the launch would drop it without a word."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivatives, reverse mode only")
+
+
 def _first_order(fn):
     """once_differentiable, without its cost where no second derivative can follow."""
     with_graph = once_differentiable(fn)
 
     def backward(ctx, *grads):
+        _no_tangents("backward", *grads)
         return with_graph(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
     return backward
 
@@ -773,6 +783,7 @@ def _attention_checks(query, key, value, scale, max_disparity, key_lengths, key_
         if key_mask.shape != (b, lk) or key_mask.dtype != torch.bool:
             raise RuntimeError(f"{what}: key_mask must be ({b}, {lk}) truth values, got "
                                f"{tuple(key_mask.shape)} {key_mask.dtype}")
+    _no_tangents(what, query, key, value)
     index = _one_device(query, key, value)
     if key_lengths is not None:
         _one_device(query, key_lengths)
@@ -805,9 +816,10 @@ def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengt
 
     D is a multiple of 8 up to 128; any strides (a copy is made where the values are not contiguous
     or rows not 16-byte aligned).  fp32, fp16 or bf16 with scores, statistics and sums in fp32; the
-    weights enter the second product rounded to the inputs' type.  Differentiable in query, key and
-    value, with the same bits on every run.  ``return_lse``: also the (B,Lq,H) fp32 logarithm of the
-    softmax's sum (-inf for an empty row; not differentiable), which joins parts of the keys.
+    weights enter the second product rounded to the inputs' type.  Differentiable once, in reverse mode,
+    in query, key and value, with the same bits on every run.  ``return_lse``: also the (B,Lq,H) fp32
+    logarithm of the softmax's sum (-inf for an empty row; not differentiable), which joins parts of the
+    keys.
     """
     if _traced():
         out, lse = _ops().cross_attention(query, key, value, key_lengths, key_mask, scale, max_disparity)
@@ -908,6 +920,7 @@ def _rotary_checks(x, positions, frequencies, layout):
         raise ValueError(f"{what}: layout must be 'half' or 'interleaved'")
     if frequencies.requires_grad:
         raise RuntimeError(f"{what}: frequencies have no gradient")
+    _no_tangents(what, x, frequencies)
     index = _one_device(x, positions, frequencies)
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
@@ -937,7 +950,7 @@ def rotary(x, positions, frequencies, layout="half", amplitude=1.0):
     the caller (``rotary_frequencies``).  ``layout``: ``"half"`` pairs value n with n + R/2,
     ``"interleaved"`` 2n with 2n + 1.  ``amplitude`` multiplies the turned values.  The angle is formed
     in 64 bits, so far positions are as exact as near ones; one rounding, to the tokens' type.
-    Differentiable in x.
+    Differentiable in x (reverse mode).
     """
     if _traced():
         return _ops().rotary(x, positions, frequencies, layout, float(amplitude))
@@ -979,6 +992,7 @@ def _norm_checks(what, x, weight, residual, eps):
             raise RuntimeError(f"{what}: x/residual shape mismatch {tuple(shape)} vs {tuple(residual.shape)}")
     if not 0.0 <= float(eps) < 3.4e38:
         raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    _no_tangents(what, x, weight, residual)
     return _one_device(x, weight) if residual is None else _one_device(x, weight, residual)
 
 
@@ -1084,7 +1098,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     residual's type, and ``(y, s)`` is returned: s is the stream that the next layer adds to, and y is
     the norm of s as it is handed on.  x is fp32, fp16 or bf16, y has its type; weight (C,) and
     residual have it or are fp32 (a 32-bit stream beside 16-bit layers).  C is 1 to 65536; sums are
-    fp32.  Differentiable in x, weight and residual (weight's gradient is summed in one order).
+    fp32.  Differentiable once, in reverse mode, in x, weight and residual (weight's gradient is summed
+    in one order).
     """
     if _traced():
         if residual is None:

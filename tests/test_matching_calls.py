@@ -124,3 +124,47 @@ def test_attention_backward_op_refuses(case, request):
     call = library._attn_backward if "device" in case else ops.cross_attention_backward
     with pytest.raises(error):
         call(q, k, k, out, lse, dout, None, mask)
+
+
+# ------------------------------------------------------------------------- forward-mode derivatives
+def _one_of_each():
+    """{name: (function of one float tensor, its shape)}: every differentiable place of every call."""
+    q, k, f, p = torch.zeros(2, 5, 4, 16), torch.zeros(2, 7, 2, 16), F.rotary_frequencies(8), torch.arange(5)
+    x, w = torch.zeros(3, 8), torch.zeros(8)
+    return {
+        "query": (lambda t: F.cross_attention(t, k, k), q), "key": (lambda t: F.cross_attention(q, t, k), k),
+        "value": (lambda t: F.cross_attention(q, k, t), k), "rotary": (lambda t: F.rotary(t, p, f), q),
+        "norm": (lambda t: F.rms_norm(t, w), x), "weight": (lambda t: F.rms_norm(x, t), w),
+        "residual": (lambda t: F.rms_norm(x, w, t), x), "e4m3": (lambda t: F.rms_norm_e4m3(t, w), x),
+        "attention op": (lambda t: ops.cross_attention(q, t, k), k), "rotary op": (lambda t: ops.rotary(t, p, f), q),
+        "norm op": (lambda t: ops.rms_norm(t, w), x), "add norm op": (lambda t: ops.add_rms_norm(x, w, t), x),
+        "e4m3 op": (lambda t: ops.rms_norm_e4m3(x, t), w)}
+
+
+@pytest.mark.parametrize("grad", [False, True], ids=["plain", "requires grad"])
+@pytest.mark.parametrize("place", list(_one_of_each()))
+def test_forward_mode_raises(place, grad, no_launch):
+    """A tangent is refused, never dropped; without one the call goes on inside a dual level.  (An op
+    whose input requires a gradient is refused by torch, once it has run.)"""
+    from torch.autograd import forward_ad
+
+    call, like = _one_of_each()[place]
+    refused = (NotImplementedError, Reached) if grad and place.endswith("op") else NotImplementedError
+    with forward_ad.dual_level():
+        with pytest.raises(refused):
+            call(forward_ad.make_dual(like.clone().requires_grad_(grad), torch.ones_like(like)))
+        with pytest.raises(Reached):
+            call(like)
+    if not place.endswith("op"):
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(call, (like,), (torch.ones_like(like),))
+
+
+def test_forward_mode_over_backward_raises():
+    from torch.autograd import forward_ad
+
+    backward = F._first_order(lambda ctx, g: (g * 2, None))
+    g = torch.ones(3)
+    assert torch.equal(backward(None, g)[0], 2 * g)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        backward(None, forward_ad.make_dual(g, g))
