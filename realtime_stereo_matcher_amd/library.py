@@ -277,10 +277,11 @@ def _attn_fake(query, key, value, key_lengths=None, key_mask=None, scale=None, m
 def _attn_setup(ctx, inputs, output):
     q, k, v, lengths, mask, scale, max_disparity = inputs
     ctx.save_for_backward(q, k, v, *output, lengths, mask)
+    ctx.mark_non_differentiable(output[1])  # lse is a constant, as in an eager call
     ctx.scale, ctx.max_disparity = scale, max_disparity
 
 
-def _attn_grad(ctx, dout, dlse):
+def _attn_grad(ctx, dout, _):
     q, k, v, out, lse, lengths, mask = ctx.saved_tensors
     dq, dk, dv = torch.ops.stereocv.cross_attention_backward(
         q, k, v, out, lse, dout, lengths, mask, ctx.scale, ctx.max_disparity)

@@ -168,3 +168,43 @@ def test_forward_mode_over_backward_raises():
     assert torch.equal(backward(None, g)[0], 2 * g)
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         backward(None, forward_ad.make_dual(g, g))
+
+
+# --------------------------------------------------------------- the logarithm of the softmax's sum
+def test_attention_op_lse_has_no_gradient():
+    """Under a compiler as in an eager call: lse is a constant, and a loss on it alone has no graph."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        q, k = (torch.empty(s, requires_grad=True) for s in ((2, 5, 4, 16), (2, 7, 2, 16)))
+        out, lse = ops.cross_attention(q, k, k)
+        assert out.requires_grad and not lse.requires_grad
+        with pytest.raises(RuntimeError, match="does not require grad"):
+            torch.autograd.grad(lse.sum(), q)
+        dq, dk = torch.autograd.grad(out.sum() + lse.sum(), (q, k))
+        assert dq.shape == q.shape and dk.shape == k.shape
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_lse_has_no_gradient(backend):
+    def net(q, k):
+        return F.cross_attention(q, k, k, return_lse=True)
+
+    torch._dynamo.reset()
+    q, k = (torch.empty(s, device="meta", requires_grad=True) for s in ((2, 5, 4, 16), (2, 7, 2, 16)))
+    out, lse = torch.compile(net, backend=backend, fullgraph=True)(q, k)
+    assert out.requires_grad and not lse.requires_grad and lse.shape == (2, 5, 4)
+    assert torch.autograd.grad(out.sum(), q)[0].shape == q.shape
+
+
+@gpu
+def test_attention_op_lse_on_the_device():
+    gen = torch.Generator().manual_seed(61)
+    q, k = (torch.randn(s, generator=gen).cuda().requires_grad_() for s in ((2, 5, 4, 16), (2, 7, 2, 16)))
+    out, lse = ops.cross_attention(q, k, k)
+    eager, elog = F.cross_attention(q, k, k, return_lse=True)
+    assert not lse.requires_grad and not elog.requires_grad
+    assert torch.equal(lse.view(2, 2, 5, 2).permute(0, 2, 1, 3).reshape(2, 5, 4), elog)
+    got = torch.autograd.grad((out * elog[..., None]).sum(), (q, k))
+    want = torch.autograd.grad((eager * elog[..., None]).sum(), (q, k))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
