@@ -1086,7 +1086,7 @@ class _AddRmsNorm(torch.autograd.Function):
         if dy is None:  # only the stream was used
             if dsummed is None:
                 return None, None, None, None
-            return dsummed.to(ctx.dtype), None, dsummed, None
+            return dsummed.to(ctx.dtype), torch.zeros_like(weight), dsummed, None
         dx, dres, dw = _norm_backward(summed.get_device(), summed, weight, dy, dsummed, ctx.dtype, ctx.eps)
         return dx, dw, dx if dres is None else dres, None
 

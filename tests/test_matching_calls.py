@@ -208,3 +208,38 @@ def test_attention_op_lse_on_the_device():
     got = torch.autograd.grad((out * elog[..., None]).sum(), (q, k))
     want = torch.autograd.grad((eager * elog[..., None]).sum(), (q, k))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------- the norm's gradients
+@pytest.mark.parametrize("used", ["y", "stream", "both"])
+@pytest.mark.parametrize("res", [torch.float16, torch.float32], ids=str)
+def test_add_rms_norm_gives_every_gradient(used, res, monkeypatch):
+    """Whichever outputs a loss uses, each input that requires a gradient has one: 0 for a weight that
+    the stream alone does not depend on, as torch.ops gives."""
+    monkeypatch.setattr(F, "_norm_checks", lambda what, x, *a: 0)
+    monkeypatch.setattr(F, "_norm_forward", lambda index, x, w, r, eps: (x * 1, r + x.to(r.dtype)))
+    monkeypatch.setattr(F, "_norm_backward", lambda index, s, w, dy, ds, dtype, eps: (
+        dy + 1, None if s.dtype == dtype else s + 1, w + 1))
+    x, w, r = (torch.ones(s, dtype=t, requires_grad=True) for s, t in
+               (((3, 8), torch.float16), ((8,), torch.float32), ((3, 8), res)))
+    y, s = F.rms_norm(x, w, r)
+    loss = {"y": y.float().sum(), "stream": s.float().sum(), "both": y.float().sum() + s.float().sum()}[used]
+    dx, dw, dr = torch.autograd.grad(loss, (x, w, r))
+    for t, g in ((x, dx), (w, dw), (r, dr)):
+        assert g.shape == t.shape and g.dtype == t.dtype
+    if used == "stream":
+        assert not dw.any()
+
+
+@gpu
+@pytest.mark.parametrize("res", [torch.float16, torch.float32], ids=str)
+def test_add_rms_norm_stream_alone(res):
+    gen = torch.Generator().manual_seed(62)
+    x, w, r = (torch.randn(s, generator=gen).to("cuda", t).requires_grad_() for s, t in
+               (((5, 40), torch.float16), ((40,), torch.float32), ((5, 40), res)))
+    g = torch.randn(5, 40, generator=gen).to("cuda", res)
+    got = torch.autograd.grad(F.rms_norm(x, w, r)[1], (x, w, r), g)
+    want = torch.autograd.grad(ops.add_rms_norm(x, w, r)[1], (x, w, r), g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    F.rms_norm(x, w, r)[1].float().sum().backward()
+    assert w.grad is not None and not w.grad.any()
