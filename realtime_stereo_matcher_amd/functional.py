@@ -1122,7 +1122,8 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
 
     q is (..., C) float8_e4m3fn, the code nearest to y / scale (formed in 64 bits); a scale is max|y| / 448
     over the row (``group=None``; scales (..., 1)) or over each 128 values of it (``group=128``; scales
-    (..., ceil(C / 128))), and 1 where y is 0.  Forward only.
+    (..., ceil(C / 128))), and 1 where y is 0.  Forward only: x and residual that require a gradient are
+    refused, and the backward pass of a weight's raises.
     """
     if group not in (None, 128):
         raise ValueError(f"rms_norm_e4m3: group must be None (a row) or 128, got {group}")
@@ -1131,7 +1132,10 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
             return _ops().rms_norm_e4m3(x, weight, float(eps), group or 0)
         return _ops().add_rms_norm_e4m3(x, weight, residual, float(eps), group or 0)
     index = _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
-    if _grads_wanted(x, weight, residual):
+    if _grads_wanted(x, residual):
         raise NotImplementedError("rms_norm_e4m3 is forward only: call it under torch.no_grad()")
-    out = _norm_forward(index, x, weight, residual, float(eps), group or 0)
-    return out[:2] if residual is None else out
+
+    def run():
+        out = _norm_forward(index, x, weight, residual, float(eps), group or 0)
+        return out[:2] if residual is None else out
+    return _ForwardOnly.apply(run, weight) if _grads_wanted(weight) else run()

@@ -243,3 +243,24 @@ def test_add_rms_norm_stream_alone(res):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     F.rms_norm(x, w, r)[1].float().sum().backward()
     assert w.grad is not None and not w.grad.any()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_e4m3_takes_trainable_weights(residual, monkeypatch):
+    """A model whose weights can be trained is evaluated outside no_grad; its backward pass raises, as
+    that of the other forward-only operators.  Rows that require a gradient are refused in the call."""
+    monkeypatch.setattr(F, "_one_device", lambda *ts: 0)
+    monkeypatch.setattr(F, "_norm_forward", lambda index, x, w, r, eps, group: (
+        x.to(torch.float8_e4m3fn), torch.ones(3, 1), None if r is None else x + r))
+    x, w = torch.ones(3, 8), torch.ones(8, requires_grad=True)
+    r = torch.ones(3, 8) if residual else None
+    got = F.rms_norm_e4m3(x, w, r)
+    assert len(got) == (3 if residual else 2) and got[0].dtype == torch.float8_e4m3fn
+    with pytest.raises(NotImplementedError):
+        (got[0].float().sum() * got[1].sum()).backward()
+    with torch.no_grad():
+        assert not F.rms_norm_e4m3(x, w, r)[0].requires_grad
+    assert not F.rms_norm_e4m3(x, w.detach(), r)[0].requires_grad
+    for rows in ((x.requires_grad_(), r), (x.detach(), torch.ones(3, 8, requires_grad=True))):
+        with pytest.raises(NotImplementedError, match="no_grad"):
+            F.rms_norm_e4m3(rows[0], w, rows[1])
