@@ -4,6 +4,7 @@ kernels may be off by, from the roundings that their types force.
 u(t) = eps(t) / 2 is the relative error of one rounding to type t (bf16 2^-8, fp16 2^-11, fp32 2^-24).
 """
 import math
+from fractions import Fraction
 
 import torch
 
@@ -92,12 +93,39 @@ def attention(q, k, v, scale, ok, dout=None):
     return val, tol
 
 
-def rotary(x, positions, frequencies, layout, amplitude=1.0, inverse=False):
+def _pi(bits):
+    """pi as a fraction, within 2^-(bits - 8): 16 atan(1/5) - 4 atan(1/239) (Machin)."""
+    def atan(n):
+        x = total = (1 << bits) // n
+        k = 1
+        while x:
+            x, k = x // (n * n), k + 2
+            total += x // k if k % 4 == 1 else -(x // k)
+        return total
+    return Fraction(16 * atan(5) - 4 * atan(239), 1 << bits)
+
+
+def wrapped(positions, frequencies):
+    """positions * frequencies modulo 2 pi, in [-pi, pi], exact up to the one rounding to 64 bits: both are
+    whole multiples of powers of two, and their product is formed as a fraction."""
+    turn = 2 * _pi(300)
+
+    def one(p, f):
+        a = Fraction(p) * Fraction(f)
+        return float(a - turn * round(a / turn))
+    rows = [[one(p, f) for f in frequencies.tolist()] for p in positions.reshape(-1).tolist()]
+    return torch.tensor(rows, dtype=torch.float64).view(*positions.shape, -1)
+
+
+def rotary(x, positions, frequencies, layout, amplitude=1.0, inverse=False, exact=False):
     """(y, bound): the turn in 64 bits; off by one rounding of y, and 2^-22 of the pair's length for
-    the fp32 angle (in turns, within 2^-26 of 1), its sine and the two products."""
+    the fp32 angle (in turns, within 2^-26 of 1), its sine and the two products.  ``exact``: the angle is
+    formed exactly (the product in 64 bits else), at whatever position."""
     r = 2 * frequencies.numel()
     a = x.detach().cpu().double()
     angle = positions.cpu().double().reshape(-1, positions.shape[-1])[:, :, None] * frequencies.cpu()
+    if exact:
+        angle = wrapped(positions.reshape(-1, positions.shape[-1]), frequencies)
     z = torch.polar(torch.full_like(angle, amplitude), -angle if inverse else angle)[:, :, None]
     one, two = (slice(0, r // 2), slice(r // 2, r)) if layout == "half" else (slice(0, r, 2), slice(1, r, 2))
     w = torch.complex(a[..., one].contiguous(), a[..., two].contiguous())

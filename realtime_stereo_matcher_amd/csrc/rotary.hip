@@ -4,9 +4,9 @@
 // "half": pair i is values i and i + R/2; "interleaved": values 2i and 2i + 1.  The values past R
 // pass through.  The gradient is the turn by -t f_i.
 //
-// The angle is formed in 64 bits as a count of turns, t (f / 2 pi), and only its fraction, in
-// [-1/2, 1/2], is rounded to fp32: a position of 2^31 is turned as exactly as position 1, and no
-// table of positions is kept or read.  A thread forms the sines of its pairs once and turns the
+// The angle is formed as a count of turns, t (f / 2 pi), in pairs of 64-bit numbers, and only its
+// fraction, in [-1/2, 1/2], is rounded to fp32: any 64-bit position is turned as exactly as position
+// 1, and no table of positions is kept or read.  A thread forms the sines of its pairs once and turns the
 // same values of several heads with them, so the arithmetic hides behind the one read and one
 // write of x that bound the operator: 4 x 8160 tokens, 16 heads of 128, 64 values turned, bf16: 267 MB
 // in 54 us (4.9 TB/s, the rate of a large copy); 16 single tokens 4.2 us.
@@ -36,6 +36,19 @@ struct Args {
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec { T v[V]; };
 
+// The fraction of (p + p0) f / (2 pi), for a p that 64 bits hold and a p0 that is small beside it.  f's
+// turns are hi + lo, within 2^-105 of them; p hi is its rounding a and the rest e.  Each part's own
+// fraction is exact, so what is lost is about 2^-53 and |p f| 2^-105.  (Twelve 64-bit operations more
+// a pair than one product has; the copy still hides them.)  Nothing may be contracted here.
+__device__ __forceinline__ float turned_part(double p, double p0, double f) {
+#pragma clang fp contract(off)
+  constexpr double kTurn = 0x1.45f306dc9c883p-3, kRest = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
+  const double hi = f * kTurn, lo = fma(f, kRest, fma(f, kTurn, -hi));
+  const double a = p * hi, e = fma(p, hi, -a), c = fma(p, lo, p0 * hi);
+  const double t = (a - rint(a)) + ((e - rint(e)) + (c - rint(c)));
+  return (float)(t - rint(t));
+}
+
 template <typename T, int V, bool HALF>
 __global__ __launch_bounds__(256) void rotate(Args a) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -58,18 +71,17 @@ __global__ __launch_bounds__(256) void rotate(Args a) {
     return;
   }
   const int64_t at = b * a.ps + t;
-  const double position = a.wide_pos ? (double)static_cast<const int64_t*>(a.pos)[at]
-                                     : (double)static_cast<const int*>(a.pos)[at];
+  const int64_t pos = a.wide_pos ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int*>(a.pos)[at];
+  // past 2^53 the last bits on their own, so that both parts are exact
+  const int64_t last = ((uint64_t)pos + (1ull << 53)) >> 54 != 0 ? pos & 2047 : 0;
+  const double p0 = (double)last, p1 = (double)(pos - last);
   // HALF: V pairs, one value of each in two vectors; interleaved: V/2 pairs side by side (V = 1:
   // a pair is two scalars in either layout)
   constexpr int P = HALF || V == 1 ? V : V / 2;
   float cs[P], sn[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
-    const double turns = position * (a.freq[col * P + p] * kTurn);
-    const float part = (float)(turns - rint(turns));
-    sincospif(2.f * part, &sn[p], &cs[p]);
+    sincospif(2.f * turned_part(p1, p0, a.freq[col * P + p]), &sn[p], &cs[p]);
     cs[p] *= a.amp;
     sn[p] *= a.amp * a.sign;
   }

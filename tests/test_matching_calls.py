@@ -264,3 +264,42 @@ def test_norm_e4m3_takes_trainable_weights(residual, monkeypatch):
     for rows in ((x.requires_grad_(), r), (x.detach(), torch.ones(3, 8, requires_grad=True))):
         with pytest.raises(NotImplementedError, match="no_grad"):
             F.rms_norm_e4m3(rows[0], w, rows[1])
+
+
+# ----------------------------------------------------------------------------------- far positions
+FAR = [0, 1, -1, 4095, -(1 << 31), (1 << 31) - 1, 1 << 31, (1 << 40) + 12345, 1 << 53, (1 << 53) + 1,
+       -(1 << 53) - 3, (1 << 62) - 77, -(1 << 62) + 999, (1 << 63) - 1, -(1 << 63)]
+
+
+def test_oracle_wraps_angles():
+    """Against the double-precision remainder where that is exact enough, and at a known far angle."""
+    f = torch.tensor([1.0, 0.37, 3.0e-3], dtype=torch.float64)
+    p = torch.tensor([0, 1, 5, -17, 1000, 65535])
+    a = p.double()[:, None] * f
+    assert ((O.wrapped(p, f) - a + 2 * math.pi * torch.round(a / (2 * math.pi))).abs() <= 1e-11).all()
+    # the C library reduces any double exactly
+    far = [710, 1 << 40, (1 << 53) - 1, 1 << 62, -(1 << 63)]
+    for p, a in zip(far, O.wrapped(torch.tensor(far), f[:1])[:, 0].tolist()):
+        assert abs(math.sin(a) - math.sin(p)) < 1e-15 and abs(math.cos(a) - math.cos(p)) < 1e-15
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize("width", [16, 10])
+def test_rotary_positions_of_any_size(width, kind, layout):
+    """A far position is turned as exactly as a near one: two 64-bit roundings at most come on top of
+    the fp32 fraction (the oracle's bound, with nothing for the distance)."""
+    positions = torch.tensor([p for p in FAR if kind == torch.int64 or -(1 << 31) <= p < 1 << 31], dtype=kind)
+    n = len(positions)
+    gen = torch.Generator().manual_seed(63)
+    x, g = torch.randn(2, n, 3, width, generator=gen), torch.randn(2, n, 3, width, generator=gen)
+    f = torch.cat((F.rotary_frequencies(width - 4), torch.tensor([2.0 * math.pi, 12.5], dtype=torch.float64)))
+    X = x.cuda().requires_grad_()
+    y = F.rotary(X, positions.cuda(), f.cuda(), layout=layout)
+    dx, = torch.autograd.grad(y, X, g.cuda())
+    for got, rows, back in ((y, x, False), (dx, g, True)):
+        want, bound = O.rotary(rows, positions, f, layout, inverse=back, exact=True)
+        off = (got.detach().cpu().double() - want).abs()
+        worst = (off / bound).amax((0, 2, 3))
+        assert bool((off <= bound).all()), dict(zip(positions.tolist(), worst.tolist()))
