@@ -44,6 +44,10 @@ template <typename T, int DP, bool FEW, int GROUPS> struct Cfg {
 };
 
 constexpr float kLazy = 8.f;
+// fp16 weights are formed times 2^7, so that with the lazy maximum they take the type's whole range (at
+// most 2^15): each is rounded within 2^-32 of the largest, where 2^-25 each was lost, which 65 thousand
+// keys far below one add up to 2e-3 of the output.  The sum of the weights carries the same factor.
+template <typename T> constexpr float kWeightUp = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 template <typename T, int DP, bool KMASK, bool FEW, int GROUPS>
 __global__ __launch_bounds__((Cfg<T, DP, FEW, GROUPS>::kThreads), (FEW || (sizeof(T) == 4 && DP == 128) ? 1 : 2))
@@ -174,7 +178,7 @@ void attn_fwd(Args a) {
         for (int r = 0; r < 16; ++r) o[db][r] *= f;
       m = mn;
     }
-    const float mc = m == -INFINITY ? 0.f : m * a.c;
+    const float mc = m == -INFINITY ? 0.f : fmaf(m, a.c, -kWeightUp<T>);
     float part_l[2] = {0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -239,7 +243,7 @@ void attn_fwd(Args a) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= inv;
-      const float lse = sum == 0.f ? -INFINITY : fmaf(from_m, a.c, __builtin_amdgcn_logf(sum)) * kLn2;
+      const float lse = sum == 0.f ? -INFINITY : fmaf(from_m, a.c, __builtin_amdgcn_logf(sum) - kWeightUp<T>) * kLn2;
       const int64_t ra = ((int64_t)b * a.KV + kv) * a.rows + grow;
       if (a.splits > 1) {
         const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + ra;
@@ -255,7 +259,7 @@ void attn_fwd(Args a) {
     if (!there) return;
     const int64_t at = ((int64_t)b * a.KV + kv) * a.rows + row;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float lse = l == 0.f ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l)) * kLn2;
+    const float lse = l == 0.f ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l) - kWeightUp<T>) * kLn2;
     if (a.splits > 1) {
       const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + at;
       store_columns<T, DP, float>(a.part_o + ps * a.D, o, inv, half, a.D);

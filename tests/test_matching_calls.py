@@ -303,3 +303,23 @@ def test_rotary_positions_of_any_size(width, kind, layout):
         off = (got.detach().cpu().double() - want).abs()
         worst = (off / bound).amax((0, 2, 3))
         assert bool((off <= bound).all()), dict(zip(positions.tolist(), worst.tolist()))
+
+
+# --------------------------------------------------------------------- attention at fp16's two ends
+@gpu
+@pytest.mark.parametrize("lq,batch", [(1, 1), (40, 1), (300, 30)])
+def test_attention_fp16_counts_small_weights(lq, batch):
+    """One key far above many: each of the others has a weight of e^-17.6875 = 2^-25.5, below half of
+    fp16's smallest step, and together they are 1.4e-3 of the output (which is all there is of it).
+    The weights enter the product times 2^7 against a running maximum, so each is off by 2^-32 at
+    most; the sum of the weights and the output's one rounding come on top."""
+    lk = 65536
+    q, k, v = torch.zeros(batch, lq, 1, 8), torch.zeros(batch, lk, 1, 8), torch.ones(batch, lk, 1, 8)
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 1.0, 17.6875, 0.0
+    out, lse = F.cross_attention(*(t.half().cuda() for t in (q, k, v)), scale=1.0, return_lse=True)
+    rest = (lk - 1) * math.exp(-17.6875)
+    want = rest / (1 + rest)
+    off = (out.cpu().double() - want).abs().max()
+    assert off <= want * (O.unit(torch.float16) + lk * O.F32) + lk * 2.0 ** -32 + O.tiny(torch.float16), float(off)
+    near_lse = 17.6875 + math.log1p(rest)
+    assert (lse.cpu().double() - near_lse).abs().max() <= (lk + 64) * O.F32 + 4 * O.F32 * near_lse
