@@ -32,7 +32,7 @@ def allowed(b, lq, lk, band=None, lengths=None, mask=None):
     return ok
 
 
-def attention(q, k, v, scale, ok, dout=None):
+def attention(q, k, v, scale, ok, dout=None, raised=0):
     """(out, lse), with ``dout`` also (dq, dk, dv), and bounds of the same shapes, as two dicts.
 
     Bounds, elementwise with p the weights, L keys, D values, u the type's unit, f = 2^-24:
@@ -43,7 +43,8 @@ def attention(q, k, v, scale, ok, dout=None):
       ds = p (g.v - delta):  p (D f sum |g||v| + sum |g| bound(out)) + |ds| (u + rp + 4 f)
       dq:        scale (sum bound(ds) |k| + L f sum |ds||k|) + u |dq|, dk and dv alike over the rows
     fp16 adds half a subnormal step for operands below the type's range: weights (times 2^14 in dv),
-    ds of rows brought to |g| <= 1 (dq) and of key heads brought to |g| <= 1 (dk).
+    ds of rows brought to |g| <= 1 (dq) and of key heads brought to |g| <= 1 (dk), there times 2^raised
+    (dq) and 2^(raised - 1) (dk): 0 is an upper bound where the range is not passed, which takes 8.
     """
     t = q.dtype
     low = t != torch.float32
@@ -81,8 +82,9 @@ def attention(q, k, v, scale, ok, dout=None):
     kmax = ge.abs().reshape(b, kv, -1).amax(-1) if ge.numel() else ge.new_zeros(b, kv)
     kmax = kmax.repeat_interleave(g, 1)[:, :, None, None]
     some = ok[:, None].double()
-    eq = scale * ((eds + sub * 2 * gmax * some) @ ke.abs() + (lk + 8) * F32 * (ds.abs() @ ke.abs()))
-    ek = scale * ((eds + sub * 2 * kmax * some).transpose(2, 3) @ qe.abs()
+    lower = 2.0 ** -raised
+    eq = scale * ((eds + sub * 2 * lower * gmax * some) @ ke.abs() + (lk + 8) * F32 * (ds.abs() @ ke.abs()))
+    ek = scale * ((eds + sub * (4 if raised else 2) * lower * kmax * some).transpose(2, 3) @ qe.abs()
                   + (lq * g + 8) * F32 * (ds.abs().transpose(2, 3) @ qe.abs()))
     ev = ((p * (uw + rp + (lq * g + 8) * F32) + sub * 2.0 ** -14 * some).transpose(2, 3) @ ge.abs())
     heads = lambda x: x.reshape(b, kv, g, lk, d).sum(2).permute(0, 2, 1, 3)  # noqa: E731

@@ -16,10 +16,13 @@
 //             sum_j p_ij k_j (one product more, on the keys already read), is taken off.  That is
 //             delta's error and, with it, the part of ds' own rounding that meets the keys' mean.
 //   attn_dkv  a wave owns 32 keys; loops over the rows of all heads that share them
-// fp16: ds would fall out of the type's range for small gradients, so g enters with a power of
-// two: one that brings the row's largest |g| into [1/2, 1) in attn_dq (a lane's scalar), the
-// largest of the whole key head in attn_dkv; p enters dv times 2^14.  The factors are exact and are
-// taken out of the fp32 sums at the end.
+// fp16: ds would fall out of the type's range, so it enters its product with a power of two: one that
+// brings the row's largest |g| into [1/2, 1) in attn_dq (a lane's scalar), the largest of the whole key
+// head in attn_dkv, and about 2^8 more, since weights and values are mostly far below 1.  Where that
+// passes the range (values of about 100 and more at large weights) the sum of the rounded ds is not
+// finite: the workgroup forms its rows once more with 2^-8, which no finite input passes
+// (|g . v - delta| <= 2 * 128 * 65504), and tells attn_dkv by the sign of its tile's maximum.  p enters
+// dv times 2^14.  The factors are exact and are taken out of the fp32 sums at the end.
 #include <algorithm>
 #include <type_traits>
 
@@ -98,6 +101,24 @@ __device__ __forceinline__ int down(float x) {
   const int e = (int)((__float_as_uint(x) >> 23) & 255);
   return e == 0 || e == 255 ? 0 : min(126 - e, 100);
 }
+
+// fp16: the powers of two that ds is formed with, first and once more
+constexpr int kUpFirst = 8, kUpAgain = -8;
+
+// whether `some` holds for a lane of the workgroup, the same answer for all its waves; `lds` is free
+// before and after
+template <int WAVES> __device__ __forceinline__ bool in_workgroup(bool some, unsigned lds, int wave, int lane) {
+  const bool mine = __any(some);
+  __syncthreads();
+  if (lane == 0) lds_put(lds + 4 * wave, (int)mine);
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) any |= lds_get<int>(lds + 4 * w);
+  __syncthreads();
+  return any != 0;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }  // not NaN either
 
 template <typename T, int DP, bool KMASK, int MODE>
 __global__ __launch_bounds__((BCfg<T, DP, MODE>::kThreads), (BCfg<T, DP, MODE>::kResident))
@@ -199,25 +220,32 @@ void attn_dq(Args a) {
   // dq, and (16-bit types) the weighted mean of the keys
   constexpr int N = sizeof(T) == 4 ? 1 : 2;
   f32x16 dq[N][DP / 32];
-  float sum = 0.f;      // of p (g . v): delta again
-  float rounded = 0.f;  // of ds as it enters the product
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
+  float sum;      // of p (g . v): delta again
+  float rounded;  // of ds as it enters the product
 
   const bool long_loop = keys.te - keys.tb >= kLongLoop;
-  int t = keys.tb + part;
-  uint64_t bits = 0;
-  int byte = 0;
-  if (t < keys.te) {
-    bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
-    copy(t, lds, bits);
-    put_mask(0, bits);
-  }
-  if (KMASK) byte = keys.byte(t + C::kParts, lane);
+  int t, byte = 0;
+  uint64_t bits;
+  int up = kScaled ? kUpFirst : 0;  // p, and with it ds and all sums, is formed times 2^up
+  float from_lse = lse2 - (float)up;
+  auto begin = [&]() __attribute__((always_inline)) {
+    sum = rounded = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
+    t = keys.tb + part;
+    bits = 0;
+    if (t < keys.te) {
+      bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
+      copy(t, lds, bits);
+      put_mask(0, bits);
+    }
+    if (KMASK) byte = keys.byte(t + C::kParts, lane);
+  };
+  begin();
   auto step = [&](auto buf) __attribute__((always_inline)) {
     constexpr int kBuf = decltype(buf)::value * C::kBufQ;
     if (C::kAlone) wait_copies(); else publish();
@@ -249,7 +277,7 @@ void attn_dq(Args a) {
         mask_block(s, a.band > 0 ? band_bits(left, token - (keys.first(t) + 32 * kb), a.band) : left, half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -from_lse));
         if constexpr (N == 2) {
           sum = fmaf(p, ds[0][r], sum);
           ds[1][r] = p;
@@ -266,14 +294,25 @@ void attn_dq(Args a) {
   };
   // every wave passes the same number of barriers: the parts' first tiles decide
   const int end = C::kAlone ? keys.te : keys.te + part;
-  while (t < end) {
-    step(std::integral_constant<int, 0>{});
-    t += C::kParts;
-    if (t >= end) break;
-    step(std::integral_constant<int, 1>{});
-    t += C::kParts;
-  }
   const unsigned base = lds_addr(smem);
+  auto over_keys = [&]() __attribute__((always_inline)) {
+    while (t < end) {
+      step(std::integral_constant<int, 0>{});
+      t += C::kParts;
+      if (t >= end) break;
+      step(std::integral_constant<int, 1>{});
+      t += C::kParts;
+    }
+  };
+  over_keys();
+  // a ds past fp16's range has left the sum of the rounded ones infinite, or NaN
+  if constexpr (kScaled)
+    if (in_workgroup<C::kWaves>(!finite(rounded), base, wave, lane)) {
+      up = kUpAgain;
+      from_lse = lse2 - (float)up;
+      begin();
+      over_keys();
+    }
   if constexpr (C::kParts > 1) __syncthreads();
   if constexpr (N == 2) {
     sum = other_half_sum(sum);
@@ -293,13 +332,23 @@ void attn_dq(Args a) {
       }
       __syncthreads();
     }
-    if (half == 0 && part == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift);
+    if constexpr (kScaled) {
+      // attn_dkv forms ds with half the factor and the exact delta, and stays in range where this was
+      // so here and delta's rounding moves ds by no more than 2^14
+      const bool near = fabsf(sum - __builtin_ldexpf(delta, up)) <= 0x1p14f;
+      if (in_workgroup<C::kWaves>(up == kUpAgain || !near, base, wave, lane) && tid == 0) {
+        float* top = a.tile_max + ((int64_t)b * a.KV + kv) * a.row_tiles + rt;
+        *top = -*top;
+      }
+    }
+    if (half == 0 && part == 0) a.row_delta[at] = __builtin_ldexpf(sum, -shift - up);
+    const float off = __builtin_ldexpf(-rounded, -up);  // against weights that carry 2^up as well
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(-rounded, dq[1][db][r], dq[0][db][r]);
+      for (int r = 0; r < 16; ++r) dq[0][db][r] = fmaf(off, dq[1][db][r], dq[0][db][r]);
   }
-  const float by = __builtin_ldexpf(a.scale, -shift);
+  const float by = __builtin_ldexpf(a.scale, -shift - up);
   if constexpr (C::kParts > 1) {
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
@@ -359,10 +408,14 @@ void attn_dkv(Args a) {
   if constexpr (kScaled) {
     const float* tm = a.tile_max + ((int64_t)b * a.KV + kv) * a.row_tiles;
     float top = 0.f;
-    for (int i = lane; i < a.row_tiles; i += 64) top = fmaxf(top, tm[i]);
+    bool far = false;
+    for (int i = lane; i < a.row_tiles; i += 64) {
+      top = fmaxf(top, fabsf(tm[i]));
+      far |= tm[i] < 0.f;
+    }
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
-    shift = __builtin_amdgcn_readfirstlane(down(top));
+    shift = __builtin_amdgcn_readfirstlane(down(top)) + (__any(far) ? kUpAgain : kUpFirst) - 1;
   }
 
   const unsigned lds = lds_addr(smem) + part * 2 * C::kBufKv;

@@ -49,7 +49,8 @@ struct Args {
   float* lse;             // (B, KV, Lq * G), natural logarithm
   float *part_o, *part_l; // split keys: (splits, B, KV, rows, D) and (splits, B, KV, rows)
   float *row_lse, *row_delta;  // backward: (B, KV, padded rows)
-  float* tile_max;        // backward, fp16: largest |dout| of each row tile, (B, KV, row tiles)
+  float* tile_max;        // backward, fp16: largest |dout| of each row tile, (B, KV, row tiles); negative
+                          // where ds passed the type's range
   const int* lengths;     // (B) or null
   const uint8_t* mask;    // (B, Lk) or null
   int64_t qs[3], ks[3], vs[3], gs[3];  // element strides of batch, token and head

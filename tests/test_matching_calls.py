@@ -9,6 +9,8 @@ from oracle import matching_oracle as O
 from realtime_stereo_matcher_amd import functional as F
 from realtime_stereo_matcher_amd import library  # noqa: F401  (registers the ops)
 
+from test_matching_ops import near, normal
+
 gpu = pytest.mark.gpu
 ops = torch.ops.stereocv
 
@@ -323,3 +325,82 @@ def test_attention_fp16_counts_small_weights(lq, batch):
     assert off <= want * (O.unit(torch.float16) + lk * O.F32) + lk * 2.0 ** -32 + O.tiny(torch.float16), float(off)
     near_lse = 17.6875 + math.log1p(rest)
     assert (lse.cpu().double() - near_lse).abs().max() <= (lk + 64) * O.F32 + 4 * O.F32 * near_lse
+
+
+def fp16_problem(batch, lq, lk, heads, kv, d, gen, v_scale, g_scale, q_scale=1.5):
+    n = lambda *s, scale: normal(gen, *s, dtype=torch.float16, scale=scale)  # noqa: E731
+    return (n(batch, lq, heads, d, scale=q_scale), n(batch, lk, kv, d, scale=1.5), n(batch, lk, kv, d, scale=v_scale),
+            n(batch, lq, heads, d, scale=g_scale))
+
+
+def fp16_gradients(q, k, v, g, scale, **how):
+    Q, K, V = (t.cuda().requires_grad_() for t in (q, k, v))
+    return torch.autograd.grad(F.cross_attention(Q, K, V, scale=scale, **how), (Q, K, V), g.cuda())
+
+
+SHAPES16 = [  # batch, query tokens, key tokens, heads, key heads, width: every launch shape of both passes
+    (1, 20, 60, 2, 1, 64), (2, 90, 200, 1, 1, 128), (2, 70, 90, 4, 2, 32), (17, 130, 140, 4, 4, 64),
+    (20, 130, 140, 4, 4, 32), (70, 130, 135, 4, 4, 64), (70, 130, 135, 4, 4, 32), (70, 65, 130, 4, 4, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("cfg", SHAPES16, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("kind", ["mask", "rows"])
+def test_attention_fp16_gradients_of_large_values(cfg, kind):
+    """Values of 40 thousand beside small gradients: p (g . v - delta), with g brought to 1, is past
+    fp16's range, and every gradient inside it.  In "rows" some rows alone pass it."""
+    b, lq, lk, h, kv, d = cfg
+    q, k, v, g = fp16_problem(*cfg, torch.Generator().manual_seed(64), 1.0, 1.0, 2.0)
+    g = g.sign() * 2.0 ** -10
+    big = (v.float() * 4e4).clamp(-6e4, 6e4).half()
+    mask = None
+    if kind == "mask":
+        v = big
+        mask = torch.rand((b, lk), generator=torch.Generator().manual_seed(65)) < 0.8
+        mask[:, 0] = True
+    else:  # those of the last sequence
+        v[-1] = big[-1]
+    scale = d ** -0.5
+    ok = O.allowed(b, lq, lk, mask=mask)
+    val, tol = O.attention(q, k, v, scale, ok, g, raised=-8)
+    gd, vd = g.double(), v.double().repeat_interleave(h // kv, 2)
+    dp = gd.permute(0, 2, 1, 3) @ vd.permute(0, 2, 3, 1).contiguous()
+    out = val["out"].permute(0, 2, 1, 3)
+    p = torch.exp(scale * (q.double().permute(0, 2, 1, 3) @ k.double().repeat_interleave(h // kv, 2).permute(0, 2, 3, 1)
+                           .contiguous()) - val["lse"].permute(0, 2, 1)[..., None])
+    ds = p * (dp - (gd.permute(0, 2, 1, 3) * out).sum(-1, keepdim=True)) * ok[:, None]
+    assert float(ds.abs().max()) * 2.0 ** 9 > 65520, "g brought to 1/2: not past the range"
+    for x in ("dq", "dk", "dv", "out"):
+        assert float(val[x].abs().max()) < 6e4, "a result out of range"
+    for n, x in zip(("dq", "dk", "dv"), fp16_gradients(q, k, v, g, scale, key_mask=None if mask is None else mask.cuda())):
+        near(x, val[n], tol[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("cfg", SHAPES16, ids=lambda c: "-".join(map(str, c)))
+def test_attention_fp16_gradients_within_range(cfg):
+    """Ordinary values: ds is formed times 2^8 (dq) and 2^7 (dk), and its bound is that much closer."""
+    b, lq, lk, h, kv, d = cfg
+    q, k, v, g = fp16_problem(*cfg, torch.Generator().manual_seed(66), 1.0, 1.0)
+    val, tol = O.attention(q, k, v, d ** -0.5, O.allowed(b, lq, lk), g, raised=8)
+    for n, x in zip(("dq", "dk", "dv"), fp16_gradients(q, k, v, g, d ** -0.5)):
+        near(x, val[n], tol[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [1, 40])
+def test_attention_fp16_gradients_over_many_keys(heads):
+    """65,536 keys of one weight, whose values are +-0.0195 in halves: with g brought to 1/2, ds is 2.5 of
+    fp16's smallest steps and was rounded to 2, in every term of dq and of dk."""
+    lk, lq, d = 65536, 5, 8
+    q, k, v, g = (torch.zeros(s) for s in ((1, lq, heads, d), (1, lk, heads, d), (1, lk, heads, d), (1, lq, heads, d)))
+    q[..., 1] = 3.0
+    k[:, : lk // 2, :, 0] = 1.0
+    v[:, : lk // 2, :, 2], v[:, lk // 2:, :, 2] = 2.5 * 2.0 ** -7, -2.5 * 2.0 ** -7
+    g[..., 2] = 1.0
+    q, k, v, g = (t.half() for t in (q, k, v, g))
+    val, tol = O.attention(q[:, :, :1], k[:, :, :1], v[:, :, :1], 1.0, O.allowed(1, lq, lk), g[:, :, :1], raised=8)
+    for n, x in zip(("dq", "dk", "dv"), fp16_gradients(q, k, v, g, 1.0)):
+        assert float(val[n].abs().max()) > 0
+        for head in range(heads):
+            near(x[:, :, head:head + 1], val[n], tol[n], (n, head))
