@@ -260,15 +260,18 @@ void attn_fwd(Args a) {
     const int64_t at = ((int64_t)b * a.KV + kv) * a.rows + row;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float lse = l == 0.f ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l) - kWeightUp<T>) * kLn2;
-    if (a.splits > 1) {
-      const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + at;
-      store_columns<T, DP, float>(a.part_o + ps * a.D, o, inv, half, a.D);
-      if (half == 0) a.part_l[ps] = lse;
-    } else {
-      store_columns<T, DP>(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + token) * a.H + head) * a.D,
-                           o, inv, half, a.D);
-      if (half == 0 && a.lse) a.lse[at] = lse;
-    }
+    // wide fp32 rows alone split their keys in this shape: the others' launches of so few workgroups
+    // have eight waves each (by_rows)
+    if constexpr (sizeof(T) == 4 && DP == 128)
+      if (a.splits > 1) {
+        const int64_t ps = (int64_t)split * a.B * a.KV * a.rows + at;
+        store_columns<T, DP, float>(a.part_o + ps * a.D, o, inv, half, a.D);
+        if (half == 0) a.part_l[ps] = lse;
+        return;
+      }
+    store_columns<T, DP>(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + token) * a.H + head) * a.D,
+                         o, inv, half, a.D);
+    if (half == 0 && a.lse) a.lse[at] = lse;
   }
 }
 

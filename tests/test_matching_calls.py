@@ -9,7 +9,7 @@ from oracle import matching_oracle as O
 from realtime_stereo_matcher_amd import functional as F
 from realtime_stereo_matcher_amd import library  # noqa: F401  (registers the ops)
 
-from test_matching_ops import near, normal
+from test_matching_ops import DTYPES, cuda, name, near, normal, problem
 
 gpu = pytest.mark.gpu
 ops = torch.ops.stereocv
@@ -404,3 +404,29 @@ def test_attention_fp16_gradients_over_many_keys(heads):
         assert float(val[n].abs().max()) > 0
         for head in range(heads):
             near(x[:, :, head:head + 1], val[n], tol[n], (n, head))
+
+
+# ------------------------------------------------------------------------------ more launch shapes
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=name)
+@pytest.mark.parametrize("cfg", [
+    (35, 130, 800, 1, 1, 128, None, "both"),    # fp32: 128 rows in four waves, and the keys split
+    (35, 130, 800, 1, 1, 96, None, "lengths"),
+    (45, 130, 520, 1, 1, 104, 300, "mask"),
+    (300, 20, 40, 2, 1, 64, None, "both"),      # many sequences of at most 32 rows
+    (400, 1, 33, 1, 1, 128, None, "lengths"),
+    (520, 32, 64, 1, 1, 32, 12, "mask"),
+], ids=lambda c: "-".join(map(str, c)))
+def test_cross_attention_more_shapes(cfg, dtype):
+    """With the output's gradient stored head by head."""
+    b, lq, lk, h, kv, d, band, kind = cfg
+    q, k, v, g, lengths, mask = problem(cfg, dtype, seed=7)
+    val, tol = O.attention(q, k, v, d ** -0.5, O.allowed(b, lq, lk, band, lengths, mask), g)
+    Q, K, V, G, LN, M = cuda(q, k, v, g, lengths, mask)
+    Q, K, V = (x.requires_grad_() for x in (Q, K, V))
+    out, lse = F.cross_attention(Q, K, V, return_lse=True, max_disparity=band, key_lengths=LN, key_mask=M)
+    near(out, val["out"], tol["out"], "out")
+    near(lse, val["lse"], tol["lse"], "lse")
+    G = G.transpose(1, 2).contiguous().transpose(1, 2)
+    for n, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (Q, K, V), G)):
+        near(x, val[n], tol[n], n)
