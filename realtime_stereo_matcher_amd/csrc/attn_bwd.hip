@@ -131,7 +131,9 @@ void attn_dq(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const unsigned id = xcd_id(), bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
+  const XcdId place(a.workgroups);
+  if (!place.there) return;
+  const unsigned id = place.id, bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
   const int rt = id - bkv * a.row_tiles, kv = bkv - b * a.KV;
   const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
   const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
@@ -376,7 +378,9 @@ void attn_dkv(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const unsigned id = xcd_id(), bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
+  const XcdId place(a.workgroups);
+  if (!place.there) return;
+  const unsigned id = place.id, bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
   const int jt = id - bkv * a.key_tiles, kv = bkv - b * a.KV;
   const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
   const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
@@ -561,7 +565,8 @@ int launch_dq(Args a, hipStream_t st) {
   const void* kern = reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK, MODE>);
   if (const int rc = ensure_lds_limit(kern, C::kLdsQ, stream_device(st), done)) return rc;
   const int64_t grid = (int64_t)a.B * a.KV * a.row_tiles;
-  attn_dq<T, DP, KMASK, MODE><<<dim3((unsigned)grid), C::kThreads, C::kLdsQ, st>>>(a);
+  a.workgroups = (unsigned)grid;
+  attn_dq<T, DP, KMASK, MODE><<<grid_of(grid), C::kThreads, C::kLdsQ, st>>>(a);
   return check_launch("cross_attention_backward dq");
 }
 
@@ -574,7 +579,8 @@ int launch_dkv(Args a, hipStream_t st) {
   a.key_tiles = (int)ceil_div(a.Lk, C::kTileRows);
   a.by_key_tiles = Divide(a.key_tiles);
   const int64_t grid = (int64_t)a.B * a.KV * a.key_tiles;
-  attn_dkv<T, DP, MODE><<<dim3((unsigned)grid), C::kThreads, C::kLdsKv, st>>>(a);
+  a.workgroups = (unsigned)grid;
+  attn_dkv<T, DP, MODE><<<grid_of(grid), C::kThreads, C::kLdsKv, st>>>(a);
   return check_launch("cross_attention_backward dk, dv");
 }
 

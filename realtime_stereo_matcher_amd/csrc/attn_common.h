@@ -59,6 +59,7 @@ struct Args {
   int pad_rows;           // rows up to a multiple of 128 (backward)
   int band;               // > 0: key j is a candidate of token i iff 0 <= i - j < band
   int splits, key_tiles;  // shares of the keys; tiles of keys (backward)
+  unsigned workgroups;    // of the launch
   Divide by_group, by_kv, by_row_tiles, by_splits, by_key_tiles;
   float scale, c;         // c = scale * log2(e): exp(scale x) = exp2(c x)
 };
@@ -484,11 +485,16 @@ __device__ __forceinline__ void store_columns(S* row, const f32x16 (&acc)[DP / 3
 }
 
 // Workgroups go to the 8 XCDs in turn; neighbours in `id` share keys and values, so each XCD gets
-// a contiguous share of the ids (its L2 then serves the re-reads).
-__device__ __forceinline__ unsigned xcd_id() {
-  const unsigned n = gridDim.x, x = blockIdx.x & 7, per = n >> 3, more = n & 7;
-  return x * per + min(x, more) + (blockIdx.x >> 3);
-}
+// a contiguous share of the ids (its L2 then serves the re-reads).  Ids past the last: not `there`.
+struct XcdId {
+  unsigned id;
+  bool there;
+  __device__ __forceinline__ explicit XcdId(unsigned n) {
+    const unsigned at = (unsigned)workgroup(), x = at & 7, per = n >> 3, more = n & 7;
+    id = x * per + min(x, more) + (at >> 3);
+    there = at < n;
+  }
+};
 
 int64_t fwd_workspace_bytes(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t KV, int64_t D);
 int64_t bwd_workspace_bytes(int64_t B, int64_t Lq, int64_t H, int64_t KV);

@@ -61,7 +61,9 @@ void attn_fwd(Args a) {
   const int part = FEW ? wave : wave >> 2;  // of the keys
   const int ctid = FEW ? lane : tid & 255, cwave0 = FEW ? 0 : (wave & 3) * 64;
 
-  const unsigned id = xcd_id();
+  const XcdId place(a.workgroups);
+  if (!place.there) return;
+  const unsigned id = place.id;
   // neighbours share the keys of a head, or (few rows) read the same tokens of neighbouring heads
   const unsigned u = FEW ? a.by_kv(id) : a.by_row_tiles(id);
   const int in_u = id - u * (FEW ? a.KV : a.row_tiles);
@@ -334,14 +336,15 @@ bool few_rows(int64_t B, int64_t KV, int64_t rows) {
 }
 
 template <typename T, int DP, bool KMASK, bool FEW, int GROUPS>
-int launch(const Args& a, hipStream_t st) {
+int launch(Args a, hipStream_t st) {
   using C = Cfg<T, DP, FEW, GROUPS>;
   static std::atomic<unsigned long long> done{0};
   const void* kern = reinterpret_cast<const void*>(&attn_fwd<T, DP, KMASK, FEW, GROUPS>);
   if (const int rc = ensure_lds_limit(kern, C::kLds, stream_device(st), done)) return rc;
   const int64_t grid = (int64_t)a.B * a.KV * a.splits * a.row_tiles;
   if (grid > 0x7fffffffll) return fail(SM_EINVAL, "cross_attention: too many row tiles");
-  attn_fwd<T, DP, KMASK, FEW, GROUPS><<<dim3((unsigned)grid), C::kThreads, C::kLds, st>>>(a);
+  a.workgroups = (unsigned)grid;
+  attn_fwd<T, DP, KMASK, FEW, GROUPS><<<grid_of(grid), C::kThreads, C::kLds, st>>>(a);
   if (const int rc = check_launch("cross_attention")) return rc;
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.B * a.KV * a.rows * (a.D / 4);

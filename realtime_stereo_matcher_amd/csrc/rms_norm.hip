@@ -126,7 +126,7 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void forward(Args a) {
   __shared__ float lds[TPR > 64 ? 4 * TPR / 64 : 1];
   int slot = 0;
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * kRowsWg + threadIdx.x / TPR;
+  const int64_t row = workgroup() * kRowsWg + threadIdx.x / TPR;
   const bool there = row < a.rows;
   float v[NV][8];
   float sq[1] = {0.f};
@@ -393,7 +393,7 @@ int launch_forward(const Args& a, bool q8, hipStream_t st) {
 #define SM_RUN(TPR, NV)                                                                          \
   {                                                                                              \
     constexpr int threads = TPR > 256 ? TPR : 256;                                               \
-    const dim3 grid((unsigned)ceil_div(a.rows, threads / TPR));                                  \
+    const dim3 grid = grid_of(ceil_div(a.rows, threads / TPR));                                  \
     if (q8) forward<T, TPR, NV, true><<<grid, threads, 0, st>>>(a);                              \
     else forward<T, TPR, NV, false><<<grid, threads, 0, st>>>(a);                                \
     return check_launch("rms_norm");                                                             \

@@ -51,7 +51,7 @@ __device__ __forceinline__ float turned_part(double p, double p0, double f) {
 
 template <typename T, int V, bool HALF>
 __global__ __launch_bounds__(256) void rotate(Args a) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = workgroup() * 256 + threadIdx.x;
   const int col = (int)(id % a.cols);
   const int64_t rest = id / a.cols;
   const int first = (int)(rest % a.par);
@@ -130,9 +130,9 @@ int launch(Args& a, bool half, hipStream_t st) {
   const int64_t grid = ceil_div(threads * par, 256);
   if (grid > 0x7fffffffll) return fail(SM_EINVAL, "rotary: too many tokens");
   if (half)
-    rotate<T, V, true><<<dim3((unsigned)grid), 256, 0, st>>>(a);
+    rotate<T, V, true><<<grid_of(grid), 256, 0, st>>>(a);
   else
-    rotate<T, V, false><<<dim3((unsigned)grid), 256, 0, st>>>(a);
+    rotate<T, V, false><<<grid_of(grid), 256, 0, st>>>(a);
   return check_launch("rotary");
 }
 

@@ -430,3 +430,61 @@ def test_cross_attention_more_shapes(cfg, dtype):
     G = G.transpose(1, 2).contiguous().transpose(1, 2)
     for n, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (Q, K, V), G)):
         near(x, val[n], tol[n], n)
+
+
+# ------------------------------------------- more threads than one side of a grid holds (2^32 and up)
+def parts(n, step):
+    return [slice(i, min(i + step, n)) for i in range(0, n, step)]
+
+
+@gpu
+def test_norm_of_a_billion_rows():
+    n = (1 << 30) + 77  # 64 rows a workgroup of 256 threads
+    x = torch.empty(n, 1, dtype=torch.float16, device="cuda")
+    gen = torch.Generator("cuda").manual_seed(67)
+    for p in parts(n, 1 << 26):
+        x[p].normal_(generator=gen)
+    w = torch.full((1,), 3.0, device="cuda")
+    y = F.rms_norm(x, w, eps=0.25)
+    for p in parts(n, 1 << 26):
+        t = x[p].double()
+        want = 3.0 * t / (t * t + 0.25).sqrt()
+        # the oracle's bound for one value a row: 10.5 roundings of fp32 and the output's
+        assert bool(((y[p].double() - want).abs() <= (11 * O.F32 + 2.0 ** -11) * want.abs() + 2.0 ** -25).all()), p
+
+
+@gpu
+def test_rotary_of_many_tokens():
+    b, l = (1 << 19) + 1, 1200  # seven threads a token
+    x = torch.empty(b, l, 1, 8, dtype=torch.float16, device="cuda")
+    gen = torch.Generator("cuda").manual_seed(68)
+    for p in parts(b, 1 << 15):
+        x[p].normal_(generator=gen)
+    f = torch.tensor([0.5], dtype=torch.float64, device="cuda")
+    pos = torch.arange(l, device="cuda")
+    y = F.rotary(x, pos, f)
+    cos, sin = (0.5 * pos.double()).cos()[:, None], (0.5 * pos.double()).sin()[:, None]
+    for p in parts(b, 1 << 15):
+        assert torch.equal(y[p][..., 2:], x[p][..., 2:]), p
+        u, v = x[p][..., 0].double(), x[p][..., 1].double()
+        far = 5 * O.F32 * (u * u + v * v).sqrt() + 2.0 ** -25
+        for got, want in ((y[p][..., 0], u * cos - v * sin), (y[p][..., 1], v * cos + u * sin)):
+            assert bool(((got.double() - want).abs() <= far + 2.0 ** -11 * want.abs()).all()), p
+
+
+@gpu
+def test_attention_of_many_sequences():
+    """17 million sequences of one token and one key: the output is the value, the value's gradient is
+    the output's, and the others' are 0 but for the roundings of g . v and delta."""
+    b = (1 << 24) + 3
+    gen = torch.Generator("cuda").manual_seed(69)
+    q, k, v, g = (torch.randn(b, 1, 1, 8, device="cuda", generator=gen).half() for _ in range(4))
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = F.cross_attention(q, k, v)
+    assert torch.equal(out, v)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), g)
+    assert torch.equal(dv, g)
+    # |g . v - delta| <= 16 f sum |g||v|, times |k| or |q| and the scale, and one rounding
+    off = 16 * O.F32 * (g.float() * v.detach().float()).abs().sum(-1, keepdim=True) * 8 ** -0.5 * 2
+    assert bool((dq.float().abs() <= off * k.detach().float().abs() + 2.0 ** -24).all())
+    assert bool((dk.float().abs() <= off * q.detach().float().abs() + 2.0 ** -24).all())
