@@ -53,7 +53,8 @@ template <typename T, int DP, int MODE> struct BCfg {
   static constexpr int kJoin = kParts > 1 ? kWaves * 32 * (DP + 4) * 4 : 0;
   static constexpr int kTilesQ = 2 * kBufQ * kParts;
   static constexpr int kMaskQ = 2 * kTile * 4 * kParts;  // 0 or -inf for each key of a buffer
-  static constexpr int kLdsQ = kJoin > kTilesQ + kMaskQ ? kJoin : kTilesQ + kMaskQ;
+  static constexpr int kFlagsQ = kJoin > kTilesQ + kMaskQ ? kJoin : kTilesQ + kMaskQ;  // fp16, two a wave
+  static constexpr int kLdsQ = kFlagsQ + (std::is_same<T, __half>::value ? 2 * 4 * kWaves : 0);
   static constexpr int kLdsKv = kJoin > 2 * kBufKv * kParts ? kJoin : 2 * kBufKv * kParts;
   // waves a SIMD: two where the accumulators leave room for them
   static constexpr int kResident = kAlone || DP == 128 || (kWide && DP == 64) ? 1 : 2;
@@ -105,17 +106,15 @@ __device__ __forceinline__ int down(float x) {
 // fp16: the powers of two that ds is formed with, first and once more
 constexpr int kUpFirst = 8, kUpAgain = -8;
 
-// whether `some` holds for a lane of the workgroup, the same answer for all its waves; `lds` is free
-// before and after
-template <int WAVES> __device__ __forceinline__ bool in_workgroup(bool some, unsigned lds, int wave, int lane) {
+// whether `some` holds for a lane of the workgroup, the same answer for all its waves, once they are all
+// here; `flags` is LDS that holds nothing else
+template <int WAVES> __device__ __forceinline__ bool in_workgroup(bool some, unsigned flags, int wave, int lane) {
   const bool mine = __any(some);
-  __syncthreads();
-  if (lane == 0) lds_put(lds + 4 * wave, (int)mine);
+  if (lane == 0) lds_put(flags + 4 * wave, (int)mine);
   __syncthreads();
   int any = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) any |= lds_get<int>(lds + 4 * w);
-  __syncthreads();
+  for (int w = 0; w < WAVES; ++w) any |= lds_get<int>(flags + 4 * w);
   return any != 0;
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }  // not NaN either
@@ -309,7 +308,7 @@ void attn_dq(Args a) {
   over_keys();
   // a ds past fp16's range has left the sum of the rounded ones infinite, or NaN
   if constexpr (kScaled)
-    if (in_workgroup<C::kWaves>(!finite(rounded), base, wave, lane)) {
+    if (in_workgroup<C::kWaves>(!finite(rounded), base + C::kFlagsQ, wave, lane)) {
       up = kUpAgain;
       from_lse = lse2 - (float)up;
       begin();
@@ -338,7 +337,7 @@ void attn_dq(Args a) {
       // attn_dkv forms ds with half the factor and the exact delta, and stays in range where this was
       // so here and delta's rounding moves ds by no more than 2^14
       const bool near = fabsf(sum - __builtin_ldexpf(delta, up)) <= 0x1p14f;
-      if (in_workgroup<C::kWaves>(up == kUpAgain || !near, base, wave, lane) && tid == 0) {
+      if (in_workgroup<C::kWaves>(up == kUpAgain || !near, base + C::kFlagsQ + 4 * C::kWaves, wave, lane) && tid == 0) {
         float* top = a.tile_max + ((int64_t)b * a.KV + kv) * a.row_tiles + rt;
         *top = -*top;
       }
