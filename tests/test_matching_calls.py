@@ -488,3 +488,45 @@ def test_attention_of_many_sequences():
     off = 16 * O.F32 * (g.float() * v.detach().float()).abs().sum(-1, keepdim=True) * 8 ** -0.5 * 2
     assert bool((dq.float().abs() <= off * k.detach().float().abs() + 2.0 ** -24).all())
     assert bool((dk.float().abs() <= off * q.detach().float().abs() + 2.0 ** -24).all())
+
+
+# ------------------------------------------------------------------------------------- compilers
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_layer(backend):
+    """A whole layer in one graph, with its gradients, on tensors without storage."""
+    import test_matching_ops as M
+
+    ins = [t.detach().requires_grad_() for t in M.layer_inputs(torch.float32, "meta")]
+    f = F.rotary_frequencies(16).to("meta")
+
+    def net(*ins):
+        return M.layer(lambda x, w, r: F.rms_norm(x, w, r), F.rotary,
+                       lambda q, k, v: F.cross_attention(q, k, v, max_disparity=12), *ins, f)
+
+    torch._dynamo.reset()
+    y, s = torch.compile(net, backend=backend, fullgraph=True)(*ins)
+    assert y.shape == s.shape == (3, 40, 32) and y.requires_grad and s.requires_grad
+    for t, g in zip(ins, torch.autograd.grad(y.sum() + s.sum(), ins)):
+        assert g.shape == t.shape and g.dtype == t.dtype
+
+
+@gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_layer_on_the_device(backend):
+    import test_matching_ops as M
+
+    f = F.rotary_frequencies(16, device="cuda")
+
+    def net(*ins):
+        return M.layer(lambda x, w, r: F.rms_norm(x, w, r), F.rotary,
+                       lambda q, k, v: F.cross_attention(q, k, v, max_disparity=12), *ins, f)
+
+    torch._dynamo.reset()
+    results = []
+    for run in (net, torch.compile(net, backend=backend, fullgraph=True)):
+        ins = M.layer_inputs(torch.float32, "cuda")
+        y, s = run(*ins)
+        results.append((y, s, *torch.autograd.grad(y.sin().sum() + s.cos().sum(), ins)))
+    for a, b in zip(*results):
+        # the same kernels; the compiler may add gradients in another order
+        assert float((a - b).norm()) <= 1e-6 * float(a.norm())
