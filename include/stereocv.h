@@ -270,7 +270,8 @@ int sm_v4_volume(const void* featL, const void* featR, void* out, int dtype,
  *   - key_mask[b * Lk + j] != 0 (bytes, contiguous (B, Lk); NULL: all), and
  *   - 0 <= i - j < max_disparity, the band of a cost volume's candidates (0: no band).
  * A row without an allowed key gives 0 (and -inf in lse).  What keys and values hold at positions
- * past the length or masked is not read.  lse: NULL or (B, KV, Lq * H / KV) float32, the natural
+ * past the length or masked is not read; inside, query, key and value (and dout) have to be finite where
+ * the band separates them from some of their 128 neighbours.  lse: NULL or (B, KV, Lq * H / KV) float32, the natural
  * logarithm of the softmax's sum, row i * (H / KV) + h % (H / KV): what the backward call needs.
  * Strides: element strides of (batch, token, head), multiples of 16 bytes (NULL: contiguous), tokens
  * less than 2^24 bytes apart; pointers 16-byte aligned.  The workspace (16-byte aligned; 0 bytes: none is used) holds partial
@@ -317,7 +318,8 @@ int sm_rotary(const void* x, const void* positions, const double* frequencies, v
 int sm_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* summed,
                 int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
                 int64_t x_stride, int64_t residual_stride, float eps, void* stream);
-/* The same with y in 8 bits: q = e4m3(y / scale), scale = max |y| / 448 over the row (group 0;
+/* The same with y in 8 bits: q = summed weight 448 / max |summed weight|, formed in 64 bits and rounded to
+ * 32 and then to e4m3, scale = max |y| / 448 over the row (group 0;
  * scales (rows, 1)) or over each 128 values (group 128; scales (rows, ceil(C / 128))); 1 where y is 0. */
 int sm_rms_norm_e4m3(const void* x, const void* residual, const void* weight, void* q, float* scales,
                      void* summed, int dtype, int residual_dtype, int weight_dtype, int64_t rows,

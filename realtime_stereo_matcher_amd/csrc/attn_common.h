@@ -490,7 +490,7 @@ struct XcdId {
   unsigned id;
   bool there;
   __device__ __forceinline__ explicit XcdId(unsigned n) {
-    const unsigned at = (unsigned)workgroup(), x = at & 7, per = n >> 3, more = n & 7;
+    const unsigned at = workgroup(), x = at & 7, per = n >> 3, more = n & 7;
     id = x * per + min(x, more) + (at >> 3);
     there = at < n;
   }

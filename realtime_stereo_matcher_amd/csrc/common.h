@@ -78,13 +78,13 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------------------- launches
-// A launch holds fewer than 2^32 threads along one side of its grid: `n` workgroups of up to 1024 threads as
-// rows of at most 2^21.  workgroup() is their index again, which the last row may carry past n.
+// A launch holds fewer than 2^32 threads along one side of its grid: `n` workgroups (less than 2^31) of up to
+// 1024 threads as rows of at most 2^21.  workgroup() is their index again, which the last row may carry past n.
 inline dim3 grid_of(int64_t n) {
   constexpr int64_t kSide = 1 << 21;
   return n <= kSide ? dim3((unsigned)n) : dim3((unsigned)kSide, (unsigned)ceil_div(n, kSide));
 }
-__device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ unsigned workgroup() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 // The device a stream belongs to (the current device for the null stream or on error).
 int stream_device(hipStream_t st);

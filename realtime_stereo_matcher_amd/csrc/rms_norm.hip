@@ -126,7 +126,7 @@ __global__ __launch_bounds__((TPR > 256 ? TPR : 256)) void forward(Args a) {
   __shared__ float lds[TPR > 64 ? 4 * TPR / 64 : 1];
   int slot = 0;
   const int t = threadIdx.x % TPR;
-  const int64_t row = workgroup() * kRowsWg + threadIdx.x / TPR;
+  const int64_t row = (int64_t)workgroup() * kRowsWg + threadIdx.x / TPR;
   const bool there = row < a.rows;
   float v[NV][8];
   float sq[1] = {0.f};

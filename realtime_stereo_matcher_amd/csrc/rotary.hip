@@ -51,7 +51,7 @@ __device__ __forceinline__ float turned_part(double p, double p0, double f) {
 
 template <typename T, int V, bool HALF>
 __global__ __launch_bounds__(256) void rotate(Args a) {
-  const int64_t id = workgroup() * 256 + threadIdx.x;
+  const int64_t id = (int64_t)workgroup() * 256 + threadIdx.x;
   const int col = (int)(id % a.cols);
   const int64_t rest = id / a.cols;
   const int first = (int)(rest % a.par);

@@ -809,10 +809,11 @@ def cross_attention(query, key, value, scale=None, max_disparity=None, key_lengt
     - ``0 <= i - j < max_disparity``: the band of candidates of a cost volume's row.
 
     A row without an allowed key gives 0.  Keys and values at positions past the length or masked are
-    never read, whatever they hold (NaN included); those inside have to be finite where the band
-    leaves them to some of 128 neighbouring rows only.  A row of a channels-last feature map is one sequence: ``feat.permute(0, 2, 3,
-    1).reshape(N * H, W, heads, C // heads)`` is a view, and with ``max_disparity`` the call is the
-    inner-product volume, its softmax over disparities and a weighted sum of values in one pass.
+    never read, whatever they hold (NaN included); those inside, and queries and gradients, have to be
+    finite where the band separates them from some of their 128 neighbours.  A row of a channels-last
+    feature map is one sequence: ``feat.permute(0, 2, 3, 1).reshape(N * H, W, heads, C // heads)`` is a
+    view, and with ``max_disparity`` the call is the inner-product volume, its softmax over disparities
+    and a weighted sum of values in one pass.
 
     D is a multiple of 8 up to 128; any strides (a copy is made where the values are not contiguous
     or rows not 16-byte aligned).  fp32, fp16 or bf16 with scores, statistics and sums in fp32; the
@@ -1120,9 +1121,9 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
     """``rms_norm`` with y in 8 bits, for a product that takes them: ``(q, scales)``, or ``(q, scales,
     s)`` with a residual, where ``y ~ q * scales``.
 
-    q is (..., C) float8_e4m3fn, the code nearest to y / scale (formed in 64 bits); a scale is max|y| / 448
-    over the row (``group=None``; scales (..., 1)) or over each 128 values of it (``group=128``; scales
-    (..., ceil(C / 128))), and 1 where y is 0.  Forward only: x and residual that require a gradient are
+    q is (..., C) float8_e4m3fn: ``s w * 448 / max|s w|``, formed in 64 bits and rounded to 32 and then to 8;
+    a scale is max|y| / 448 (rounded to fp32 by itself) over the row (``group=None``; scales (..., 1)) or
+    over each 128 values of it (``group=128``; scales (..., ceil(C / 128))), and 1 where y is 0.  Forward only: x and residual that require a gradient are
     refused, and the backward pass of a weight's raises.
     """
     if group not in (None, 128):
@@ -1134,8 +1135,6 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6, group=None):
     index = _norm_checks("rms_norm_e4m3", x, weight, residual, eps)
     if _grads_wanted(x, residual):
         raise NotImplementedError("rms_norm_e4m3 is forward only: call it under torch.no_grad()")
-
-    def run():
-        out = _norm_forward(index, x, weight, residual, float(eps), group or 0)
-        return out[:2] if residual is None else out
-    return _ForwardOnly.apply(run, weight) if _grads_wanted(weight) else run()
+    args = index, x, weight, residual, float(eps), group or 0
+    out = _ForwardOnly.apply(lambda: _norm_forward(*args), weight) if _grads_wanted(weight) else _norm_forward(*args)
+    return out[:2] if residual is None else out
