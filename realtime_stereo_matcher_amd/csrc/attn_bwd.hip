@@ -130,9 +130,7 @@ void attn_dq(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const XcdId place(a.workgroups);
-  if (!place.there) return;
-  const unsigned id = place.id, bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
+  const unsigned id = xcd_id(a), bkv = a.by_row_tiles(id), b = a.by_kv(bkv);
   const int rt = id - bkv * a.row_tiles, kv = bkv - b * a.KV;
   const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
   const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
@@ -221,24 +219,20 @@ void attn_dq(Args a) {
   // dq, and (16-bit types) the weighted mean of the keys
   constexpr int N = sizeof(T) == 4 ? 1 : 2;
   f32x16 dq[N][DP / 32];
-  float sum;      // of p (g . v): delta again
-  float rounded;  // of ds as it enters the product
+  float sum = 0.f;      // of p (g . v): delta again
+  float rounded = 0.f;  // of ds as it enters the product
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
 
   const bool long_loop = keys.te - keys.tb >= kLongLoop;
-  int t, byte = 0;
-  uint64_t bits;
-  int up = kScaled ? kUpFirst : 0;  // p, and with it ds and all sums, is formed times 2^up
-  float from_lse = lse2 - (float)up;
-  auto begin = [&]() __attribute__((always_inline)) {
-    sum = rounded = 0.f;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
-    t = keys.tb + part;
-    bits = 0;
+  int t = keys.tb + part;
+  uint64_t bits = 0;
+  int byte = 0;
+  auto fetch_first = [&]() __attribute__((always_inline)) {
     if (t < keys.te) {
       bits = KMASK ? __ballot(keys.byte(t, lane)) : keys.by_length(t);
       copy(t, lds, bits);
@@ -246,7 +240,9 @@ void attn_dq(Args a) {
     }
     if (KMASK) byte = keys.byte(t + C::kParts, lane);
   };
-  begin();
+  fetch_first();
+  int up = kScaled ? kUpFirst : 0;  // p, and with it ds and all sums, is formed times 2^up
+  float from_lse = lse2 - (float)up;
   auto step = [&](auto buf) __attribute__((always_inline)) {
     constexpr int kBuf = decltype(buf)::value * C::kBufQ;
     if (C::kAlone) wait_copies(); else publish();
@@ -295,24 +291,35 @@ void attn_dq(Args a) {
   };
   // every wave passes the same number of barriers: the parts' first tiles decide
   const int end = C::kAlone ? keys.te : keys.te + part;
+  while (t < end) {
+    step(std::integral_constant<int, 0>{});
+    t += C::kParts;
+    if (t >= end) break;
+    step(std::integral_constant<int, 1>{});
+    t += C::kParts;
+  }
   const unsigned base = lds_addr(smem);
-  auto over_keys = [&]() __attribute__((always_inline)) {
-    while (t < end) {
-      step(std::integral_constant<int, 0>{});
-      t += C::kParts;
-      if (t >= end) break;
-      step(std::integral_constant<int, 1>{});
-      t += C::kParts;
-    }
-  };
-  over_keys();
   // a ds past fp16's range has left the sum of the rounded ones infinite, or NaN
   if constexpr (kScaled)
     if (in_workgroup<C::kWaves>(!finite(rounded), base + C::kFlagsQ, wave, lane)) {
       up = kUpAgain;
       from_lse = lse2 - (float)up;
-      begin();
-      over_keys();
+      sum = rounded = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dq[n][db][r] = 0.f;
+      t = keys.tb + part;
+      fetch_first();
+      while (t < end) {
+        step(std::integral_constant<int, 0>{});
+        t += C::kParts;
+        if (t >= end) break;
+        step(std::integral_constant<int, 1>{});
+        t += C::kParts;
+      }
     }
   if constexpr (C::kParts > 1) __syncthreads();
   if constexpr (N == 2) {
@@ -377,9 +384,7 @@ void attn_dkv(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const XcdId place(a.workgroups);
-  if (!place.there) return;
-  const unsigned id = place.id, bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
+  const unsigned id = xcd_id(a), bkv = a.by_key_tiles(id), b = a.by_kv(bkv);
   const int jt = id - bkv * a.key_tiles, kv = bkv - b * a.KV;
   const int set = C::kAlone ? 0 : wave & 3, part = C::kAlone ? wave : wave >> 2;
   const int ctid = C::kAlone ? lane : tid & 255, cwave0 = C::kAlone ? 0 : 64 * set;
@@ -564,9 +569,9 @@ int launch_dq(Args a, hipStream_t st) {
   const void* kern = reinterpret_cast<const void*>(&attn_dq<T, DP, KMASK, MODE>);
   if (const int rc = ensure_lds_limit(kern, C::kLdsQ, stream_device(st), done)) return rc;
   const int64_t grid = (int64_t)a.B * a.KV * a.row_tiles;
-  a.workgroups = (unsigned)grid;
-  attn_dq<T, DP, KMASK, MODE><<<grid_of(grid), C::kThreads, C::kLdsQ, st>>>(a);
-  return check_launch("cross_attention_backward dq");
+  return launch_all(a, grid, "cross_attention_backward dq", [&](dim3 part) {
+    attn_dq<T, DP, KMASK, MODE><<<part, C::kThreads, C::kLdsQ, st>>>(a);
+  });
 }
 
 template <typename T, int DP, int MODE>
@@ -578,9 +583,9 @@ int launch_dkv(Args a, hipStream_t st) {
   a.key_tiles = (int)ceil_div(a.Lk, C::kTileRows);
   a.by_key_tiles = Divide(a.key_tiles);
   const int64_t grid = (int64_t)a.B * a.KV * a.key_tiles;
-  a.workgroups = (unsigned)grid;
-  attn_dkv<T, DP, MODE><<<grid_of(grid), C::kThreads, C::kLdsKv, st>>>(a);
-  return check_launch("cross_attention_backward dk, dv");
+  return launch_all(a, grid, "cross_attention_backward dk, dv", [&](dim3 part) {
+    attn_dkv<T, DP, MODE><<<part, C::kThreads, C::kLdsKv, st>>>(a);
+  });
 }
 
 // `wgs`: workgroups of 128 rows.  Up to a quarter of the compute units: 32-row workgroups (8 x 255 x 301

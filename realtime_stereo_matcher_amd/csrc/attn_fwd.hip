@@ -61,9 +61,7 @@ void attn_fwd(Args a) {
   const int part = FEW ? wave : wave >> 2;  // of the keys
   const int ctid = FEW ? lane : tid & 255, cwave0 = FEW ? 0 : (wave & 3) * 64;
 
-  const XcdId place(a.workgroups);
-  if (!place.there) return;
-  const unsigned id = place.id;
+  const unsigned id = xcd_id(a);
   // neighbours share the keys of a head, or (few rows) read the same tokens of neighbouring heads
   const unsigned u = FEW ? a.by_kv(id) : a.by_row_tiles(id);
   const int in_u = id - u * (FEW ? a.KV : a.row_tiles);
@@ -343,9 +341,9 @@ int launch(Args a, hipStream_t st) {
   if (const int rc = ensure_lds_limit(kern, C::kLds, stream_device(st), done)) return rc;
   const int64_t grid = (int64_t)a.B * a.KV * a.splits * a.row_tiles;
   if (grid > 0x7fffffffll) return fail(SM_EINVAL, "cross_attention: too many row tiles");
-  a.workgroups = (unsigned)grid;
-  attn_fwd<T, DP, KMASK, FEW, GROUPS><<<grid_of(grid), C::kThreads, C::kLds, st>>>(a);
-  if (const int rc = check_launch("cross_attention")) return rc;
+  if (const int rc = launch_all(a, grid, "cross_attention", [&](dim3 part) {
+        attn_fwd<T, DP, KMASK, FEW, GROUPS><<<part, C::kThreads, C::kLds, st>>>(a);
+      })) return rc;
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.B * a.KV * a.rows * (a.D / 4);
     attn_join<T><<<dim3((unsigned)ceil_div(n, 256)), 256, 0, st>>>(a);
