@@ -545,3 +545,52 @@ def test_attention_fp16_gradients_of_values_far_from_zero(cfg):
     for n, x in zip(("dq", "dk", "dv"), fp16_gradients(q, k, v, g, d ** -0.5)):
         assert bool(x.isfinite().all())
         near(x, val[n], tol[n], n)
+
+
+# ------------------------------------------------------------------------------- graphs and streams
+@gpu
+def test_operators_in_one_graph():
+    """Norm, rotary positions, attention and the 8-bit norm with all gradients, captured once and replayed
+    with ordinary, large (fp16's second range) and small values between eager calls; and on another stream."""
+    f = F.rotary_frequencies(32, device="cuda")
+    w = normal(torch.Generator().manual_seed(71), 64).cuda()
+    pos = torch.arange(40, device="cuda") * 1000
+
+    def step(x, r, k, v, g, z):
+        x, r, k, v, wt = leaves = [t.detach().requires_grad_() for t in (x, r, k, v, w)]
+        y, s = F.rms_norm(x, wt, r)
+        q = F.rotary(y.unflatten(-1, (2, 32)), pos, f)
+        o = F.cross_attention(q, k, v, max_disparity=24)
+        grads = torch.autograd.grad((o, s), leaves, (g, z))
+        with torch.no_grad():
+            return (o, s, *grads, *F.rms_norm_e4m3(o.flatten(2), w, s, group=128))
+
+    def inputs(seed, scale):
+        gen = torch.Generator().manual_seed(seed)
+        n = lambda *s, scale=1.0: normal(gen, *s, dtype=torch.float16, scale=scale).cuda()  # noqa: E731
+        return [n(3, 40, 64), n(3, 40, 64), n(3, 47, 2, 32, scale=2.0), n(3, 47, 2, 32, scale=scale).clamp(-6e4, 6e4),
+                n(3, 40, 2, 32, scale=2.0 ** -10), n(3, 40, 64)]
+
+    sets = [inputs(72, 1.0), inputs(73, 4e4), inputs(74, 1e-3)]
+    static = [t.clone() for t in sets[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*static)
+    same = lambda a, b: torch.equal(a.view(torch.uint8), b.view(torch.uint8))  # noqa: E731
+    for n in (0, 1, 2, 0, 1):
+        for x, y in zip(static, sets[n]):
+            x.copy_(y)
+        graph.replay()
+        want = step(*sets[n])
+        torch.cuda.synchronize()
+        assert all(bool(t.float().isfinite().all()) for t in want)
+        assert all(same(a.contiguous(), b.contiguous()) for a, b in zip(held, want)), n
+    with torch.cuda.stream(side):
+        other = step(*sets[1])
+    side.synchronize()
+    assert all(same(a.contiguous(), b.contiguous()) for a, b in zip(other, step(*sets[1])))
